@@ -26,6 +26,10 @@ EPI_STORE, EPI_BIAS, EPI_DEMOD, EPI_ACCUM, EPI_SCALE = 0, 1, 2, 3, 4
 CONV_FWD, CONV_DGRAD, CONV_WGRAD = 0, 1, 2
 ACT_SIGMOID, ACT_TANH, ACT_LEAKY = 0, 1, 2
 MATH_F32, MATH_BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 2                                # element types (GANAMD_F32 ...)
+NORM_ROWS, NORM_PLANES = 0, 1                           # ganamd_norm_desc.layout
+NORM_NONE, NORM_SILU, NORM_LEAKY, NORM_PRELU = 0, 1, 2, 3   # ganamd_norm_desc.act
+NORM_L2, NORM_MAX = 0, 1                                # kinds of gradient norm
 KERNEL_PATCH_FWD, KERNEL_PATCH_DGRAD, KERNEL_WGRAD_ROW, KERNEL_SMALL = 1, 2, 4, 8   # ganamd_conv_desc.kernel_off bits
 
 
@@ -33,6 +37,13 @@ class ConvDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in
                 ("B", "Cin", "H", "W", "Cout", "OH", "OW", "KH", "KW", "stride", "pad", "pad_mode", "transposed",
                  "packed_w", "math", "kernel_off")]
+
+
+class NormDesc(ctypes.Structure):
+    """ganamd_norm_desc (include/ganamd.h)."""
+    _fields_ = [("L", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("B", "C", "G", "layout", "dtype", "param_dtype", "act")] + \
+               [("slope", ctypes.c_float), ("eps", ctypes.c_float)]
 
 
 class GTile(ctypes.Structure):
@@ -110,6 +121,16 @@ _SIGS = {
     "ganamd_segment_sumsq": (c_int, [vp, c_long, c_int, vp, vp]),
     "ganamd_adamw": (c_int, [vp, vp, vp, vp, c_long, vp, c_float, c_float, c_float, c_float, c_float, vp]),
     "ganamd_grouped_gemm": (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, vp]),
+    "ganamd_group_norm_workspace": (c_int, [ctypes.POINTER(NormDesc), c_int, ctypes.POINTER(c_size_t)]),
+    "ganamd_group_norm_plan_info": (c_int, [ctypes.POINTER(NormDesc), c_int, ctypes.POINTER(ctypes.c_int)]),
+    "ganamd_group_norm_fwd": (c_int, [ctypes.POINTER(NormDesc), vp, vp, vp, vp, vp, vp, vp, c_size_t, vp]),
+    "ganamd_group_norm_bwd": (c_int, [ctypes.POINTER(NormDesc)] + [vp] * 10 + [c_int, vp, c_size_t, vp]),
+    "ganamd_group_norm_bwd_bwd": (c_int, [ctypes.POINTER(NormDesc)] + [vp] * 15 + [c_int, vp, c_size_t, vp]),
+    "ganamd_grad_norm_workspace": (c_size_t, [vp, c_int]),
+    "ganamd_grad_norm": (c_int, [vp, c_int, c_int, vp, vp, c_size_t, vp]),
+    "ganamd_grad_clip": (c_int, [vp, c_int, c_int, c_float, vp, vp, c_size_t, vp]),
+    "ganamd_adamw_clip_workspace": (c_size_t, []),
+    "ganamd_adamw_clip": (c_int, [vp, vp, vp, vp, c_long, vp] + [ctypes.c_double] * 5 + [c_float, vp, vp, c_size_t, vp]),
     "ganamd_prelu_tangent": (c_int, [vp, vp, vp, vp, c_int, c_long, vp, vp, c_int, vp, c_size_t, vp]),
     "ganamd_act_fwd": (c_int, [c_int, vp, c_long, c_float, vp, vp]),
     "ganamd_act_bwd": (c_int, [c_int, vp, vp, c_long, c_float, vp, vp]),

@@ -1,0 +1,946 @@
+// Group norm with its activation for gfx950: forward, backward and the backward's own backward
+// (the gradient penalty), over channels-last maps x[b][l][c] and over channel rows x[c][b][l].
+//
+// For a sample b and a group of Cg channels, N = L * Cg values, with d = x - mean:
+//   xh = d * r, r = (var + eps)^-1/2, z = xh * w[c] + b[c], y = a(z)
+//   backward:  g = gy a'(z), u = w g:   gx = r (u - m(u) - xh m(u xh)),
+//              gw = sum g xh, gb = sum g, gslope = sum gy z [z <= 0]           (m: mean over the group)
+//   double backward, v the cotangent of gx, (cw, cb, cs) those of gw, gb, gslope:
+//              q = r (v - m(v) - xh m(v xh)),  h = w q + cw xh + cb
+//              t = gy a''(z) h + cs gy [z <= 0],  e = t w + g cw - r (v m(u xh) + u m(v xh))
+//              g_gy = a'(z) h + cs z [z <= 0]
+//              g_x = r (e - m(e) - xh m(e xh)) - r xh m(u q)
+//              g_w = sum g q + t xh,  g_b = sum t,  g_slope = sum gy h [z <= 0]
+// Every group mean above is a combination of per-channel sums over l that need no other mean, so
+// each operator is ONE reduction over its inputs (5 to 10 sums a channel) and one elementwise pass
+// whose result is linear in (g, v, d, t, 1) with per-channel coefficients.
+//
+// Statistics are summed and kept in 64 bits: the sign of z selects the branch of a kinked
+// activation, and at fp32 accuracy a handful of values per 10^7 fall on the wrong side, each an
+// error of the size of the gradient.  The test itself is one fp32 comparison of x with the
+// channel's threshold (the smallest float whose z is positive), exact for every x.
+//
+// What bounds them: memory.  Two forms:
+//  * resident: one block holds all of a group's (rows: a tile of whole groups') values in
+//    registers between the reduction and the elementwise part: each input is read once.
+//  * split: the positions of a sample are cut over blocks; per-channel partials go to the
+//    workspace, a small kernel folds them, a second pass over the data writes the result.
+// No atomics: results are the same on every run.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/ganamd.h"
+
+namespace gn {
+
+enum { FWD = 0, BWD = 1, DBL = 2 };
+enum { SILU = 0, KINK = 1, SLOPE = 2 };   // SLOPE: a kinked activation whose slope has a gradient
+
+// One operator call on one batch slice, as the kernels see it.
+struct Args {
+  const void *x, *gy, *v;                       // data, in T
+  void *o1, *o2;                                // y | gx | g_gy, g_x
+  const void *w, *b, *slope, *cw, *cb, *cs;     // per-channel parameters and cotangents (pdt); may be null
+  double* stats;                                // [B][G][2]: mean, r (written by FWD)
+  double* coef;                                 // [B][G][8]: group coefficients of the elementwise pass
+  float* part;                                  // [B][S][K][C] partial sums (FWD: doubles [B][S][2][C])
+  float* par;                                   // [3][B][C]: each sample's terms of gw, gb, gslope
+  float cslope;                                 // constant slope where slope is null
+  float eps;
+  long L, B;                                    // positions, samples of the whole tensor (strides)
+  int b0;                                       // first sample of this slice
+  int C, G, Cg, pdt;
+  int TX, P;                                    // threads across the channels (rows) / planes per block; positions in flight
+  int CT, nct;                                  // channels per tile, tiles
+  int S;                                        // chunks of a sample's positions
+  int per;                                      // positions (planes: vectors) per chunk
+};
+
+// ------------------------------------------------------------------ types
+struct bf16 { uint16_t u; };
+struct f16 { _Float16 h; };
+
+__device__ __forceinline__ float up(float x) { return x; }
+__device__ __forceinline__ float up(bf16 x) { return __uint_as_float((uint32_t)x.u << 16); }
+__device__ __forceinline__ float up(f16 x) { return (float)x.h; }
+template <class T>
+__device__ __forceinline__ T down(float x);
+template <>
+__device__ __forceinline__ float down<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16 down<bf16>(float x) {
+  const __bf16 h = (__bf16)x;   // round to nearest even
+  return bf16{__builtin_bit_cast(uint16_t, h)};
+}
+template <>
+__device__ __forceinline__ f16 down<f16>(float x) { return f16{(_Float16)x}; }
+
+// V elements as the 32-bit words they come in, loaded and stored whole at any element alignment
+// (rows of an odd channel count start anywhere; global memory takes unaligned vectors).  They are
+// unpacked where they are used: a value kept for a second use stays packed.
+template <int BYTES, int ALIGN>
+struct Word;
+#define GN_WORD(BYTES, TYPE, ALIGN) \
+  template <> struct Word<BYTES, ALIGN> { typedef TYPE type __attribute__((aligned(ALIGN))); };
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+GN_WORD(16, u32x4, 4) GN_WORD(16, u32x4, 2) GN_WORD(8, u32x2, 4) GN_WORD(8, u32x2, 2)
+GN_WORD(4, uint32_t, 4) GN_WORD(4, uint32_t, 2) GN_WORD(2, uint16_t, 2)
+#undef GN_WORD
+
+template <class T, int V>
+struct Vec {
+  static constexpr int N = (V * (int)sizeof(T) + 3) / 4, PER = 4 / (int)sizeof(T);
+  typedef typename Word<sizeof(T) * V, sizeof(T)>::type W;
+  uint32_t w[N];
+  __device__ __forceinline__ float get(int j) const;
+  __device__ __forceinline__ void put(const float (&f)[V]);
+  // elements j < n become zero
+  __device__ __forceinline__ void zero_front(int n) {
+    if (n <= 0) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (PER == 1) {
+        if (i < n) w[i] = 0;
+      } else {
+        const int k = n - 2 * i;
+        w[i] = k >= 2 ? 0u : k == 1 ? w[i] & 0xffff0000u : w[i];
+      }
+    }
+  }
+  // the compiler may not carry anything derived from these words past here
+  __device__ __forceinline__ void pin() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(w[i]));
+  }
+};
+template <class T> __device__ __forceinline__ float up_bits(uint32_t w, int half);
+template <> __device__ __forceinline__ float up_bits<float>(uint32_t w, int) { return __uint_as_float(w); }
+template <> __device__ __forceinline__ float up_bits<bf16>(uint32_t w, int half) {
+  return __uint_as_float(half ? w & 0xffff0000u : w << 16);
+}
+template <> __device__ __forceinline__ float up_bits<f16>(uint32_t w, int half) {
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)(half ? w >> 16 : w));
+}
+template <class T> __device__ __forceinline__ uint32_t bits(T x);
+template <> __device__ __forceinline__ uint32_t bits<float>(float x) { return __float_as_uint(x); }
+template <> __device__ __forceinline__ uint32_t bits<bf16>(bf16 x) { return x.u; }
+template <> __device__ __forceinline__ uint32_t bits<f16>(f16 x) { return __builtin_bit_cast(uint16_t, x.h); }
+
+template <class T, int V>
+__device__ __forceinline__ float Vec<T, V>::get(int j) const { return up_bits<T>(w[j / PER], j % PER); }
+template <class T, int V>
+__device__ __forceinline__ void Vec<T, V>::put(const float (&f)[V]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    w[i] = bits(down<T>(f[i * PER]));
+    if (PER == 2 && i * PER + 1 < V) w[i] |= bits(down<T>(f[i * PER + 1 < V ? i * PER + 1 : 0])) << 16;
+  }
+}
+
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> load(const T* p) {
+  typedef typename Vec<T, V>::W W;
+  const W x = *reinterpret_cast<const W*>(p);
+  Vec<T, V> v;
+  if constexpr (sizeof(x) < 4)
+    v.w[0] = x;
+  else
+    __builtin_memcpy(v.w, &x, sizeof(x));
+  return v;
+}
+template <class T, int V>
+__device__ __forceinline__ void store(T* p, const Vec<T, V>& v, int skip) {
+  typedef typename Vec<T, V>::W W;
+  if (skip == 0) {
+    W x;
+    if constexpr (sizeof(x) < 4)
+      x = (W)v.w[0];
+    else
+      __builtin_memcpy(&x, v.w, sizeof(x));
+    *reinterpret_cast<W*>(p) = x;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j >= skip) {
+        const uint32_t h = v.w[j / Vec<T, V>::PER] >> (16 * (j % Vec<T, V>::PER));
+        if constexpr (sizeof(T) == 4)
+          reinterpret_cast<uint32_t*>(p)[j] = h;
+        else
+          reinterpret_cast<uint16_t*>(p)[j] = (uint16_t)h;
+      }
+  }
+}
+
+__device__ __forceinline__ float loadp(const void* p, int dt, long i) {
+  if (dt == GANAMD_F32) return static_cast<const float*>(p)[i];
+  if (dt == GANAMD_BF16) return up(static_cast<const bf16*>(p)[i]);
+  return up(static_cast<const f16*>(p)[i]);
+}
+
+// ------------------------------------------------------------------ which elements a thread owns
+// rows (channels last): V consecutive channels, every P-th position.  planes (channel rows): one
+// channel, every P-th vector of V positions.  The last vector of a row / plane is moved back to end
+// with it; its first `skip` elements belong to its neighbour and count as zero here.
+template <bool ROWS, int V>
+struct Map {
+  long base, step;     // element offset of position 0, of one position
+  long last;           // planes: L - V
+  int ch;              // first channel of this thread
+  int slot;            // ch within the tile
+  int p;               // first position
+  int npos;            // positions (planes: vectors) of a sample
+  int skip0;
+  bool active;
+
+  __device__ __forceinline__ Map(const Args& a, long b, int tile) {
+    const int c0 = tile * a.CT, wid = min(a.CT, a.C - c0);
+    if (ROWS) {
+      const int tx = threadIdx.x % a.TX;
+      p = threadIdx.x / a.TX;
+      const int cv = c0 + tx * V;
+      active = tx * V < wid && p < a.P;
+      ch = max(min(cv, c0 + wid - V), 0);
+      skip0 = cv - ch;
+      slot = ch - c0;
+      base = b * a.L * a.C + ch;
+      step = a.C;
+      last = 0;
+      npos = (int)a.L;
+    } else {
+      p = threadIdx.x % a.P;
+      slot = threadIdx.x / a.P;
+      ch = min(c0 + slot, a.C - 1);
+      active = slot < wid;
+      skip0 = 0;
+      base = ((long)ch * a.B + b) * a.L;
+      step = V;
+      last = a.L - V;
+      npos = (int)((a.L + V - 1) / V);
+    }
+  }
+  __device__ __forceinline__ long at(long i, int& skip) const {
+    if (ROWS) {
+      skip = skip0;
+      return base + i * step;
+    }
+    const long l = i * V, s = l < last ? l : last;
+    skip = (int)(l - s);
+    return base + s;
+  }
+};
+
+// ------------------------------------------------------------------ per-channel constants
+__device__ __forceinline__ float kink(double mean, double rw, double b, bool& neg) {
+  const float a = (float)rw;
+  neg = a < 0.f;
+  if (a == 0.f) return b > 0.0 ? -INFINITY : NAN;      // z = b whatever x is
+  const double x0 = neg ? b / rw - mean : mean - b / rw;
+  const float t = (float)x0;
+  return (double)t <= x0 ? nextafterf(t, INFINITY) : t;
+}
+
+// What the activation needs of a channel: d = x - mf; z = d * a + o (o carries the part of the
+// mean below fp32); the kink's threshold on x (on -x where a < 0), and its slope.
+template <int ACT>
+struct Chan {
+  float mf, a, o, tf, k;
+  bool neg;
+  double xo;          // xh = r d + xo
+  __device__ __forceinline__ void set(const Args& g, double mean, double r, int c) {
+    const float w = g.w ? loadp(g.w, g.pdt, c) : 1.f, bb = g.b ? loadp(g.b, g.pdt, c) : 0.f;
+    mf = (float)mean;
+    const double rw = r * (double)w;
+    xo = ((double)mf - mean) * r;
+    a = (float)rw;
+    o = (float)((double)bb + xo * (double)w);
+    k = 1.f;
+    tf = 0.f;
+    neg = false;
+    if (ACT != SILU) {
+      k = g.slope ? loadp(g.slope, g.pdt, c) : g.cslope;
+      tf = kink(mean, rw, (double)bb, neg);
+    }
+  }
+};
+
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+
+template <int ACT>
+__device__ __forceinline__ float act_fwd(const Chan<ACT>& c, float x) {
+  const float z = (x - c.mf) * c.a + c.o;
+  if (ACT == SILU) return z * sigmoid(z);
+  return z > 0.f ? z : c.k * z;
+}
+// g = gy a'(z); t = gy a''(z) (SILU) or gy [z <= 0] (kinked); z itself
+template <int ACT>
+__device__ __forceinline__ void act_bwd(const Chan<ACT>& c, float x, float d, float gy, float& g, float& t, float& z) {
+  z = d * c.a + c.o;
+  if (ACT == SILU) {
+    const float s = sigmoid(z), n = 1.f - s;
+    g = gy * (s * (1.f + z * n));
+    t = gy * (s * n * (2.f + z * (n - s)));
+  } else {
+    const bool pos = (c.neg ? -x : x) >= c.tf;
+    g = pos ? gy : c.k * gy;
+    t = pos ? 0.f : gy;
+  }
+}
+template <int ACT>
+__device__ __forceinline__ float act_d1(const Chan<ACT>& c, float x, float z) {
+  if (ACT == SILU) {
+    const float s = sigmoid(z);
+    return s * (1.f + z * (1.f - s));
+  }
+  return (c.neg ? -x : x) >= c.tf ? 1.f : c.k;
+}
+
+// ------------------------------------------------------------------ sums over positions
+// FWD sums in double (x, x^2); the others in fp32 over a thread's own positions.
+//   BWD: g, g d (, gy z [z<=0]).   DBL: v, v d, g, g d, g v, then
+//   SILU: k, k d, k d^2, k v, k v d with k = gy a''; SLOPE: s, s d, s v with s = gy [z <= 0]
+template <int MODE, int ACT>
+struct Sums {
+  static constexpr int K = MODE == FWD ? 2 : MODE == BWD ? (ACT == SLOPE ? 3 : 2)
+                                                         : (ACT == SILU ? 10 : ACT == SLOPE ? 8 : 5);
+};
+template <int MODE>
+struct AccT { typedef float type; };
+template <>
+struct AccT<FWD> { typedef double type; };
+
+template <int MODE, int ACT, bool ROWS, class T, int V, int NC, int K, class A>
+__device__ __forceinline__ void accumulate(A (&acc)[K][NC], const Chan<ACT> (&ch)[NC], const Vec<T, V>& x,
+                                           const Vec<T, V>& gy, const Vec<T, V>& v) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = ROWS ? j : 0;
+    const float xf = x.get(j);
+    if constexpr (MODE == FWD) {
+      const double xd = (double)xf;
+      acc[0][c] += xd;
+      acc[1][c] = fma(xd, xd, acc[1][c]);
+    } else {
+      const float d = xf - ch[c].mf;
+      float g, t, z;
+      act_bwd<ACT>(ch[c], xf, d, gy.get(j), g, t, z);
+      if constexpr (MODE == BWD) {
+        acc[0][c] += g;
+        acc[1][c] = fmaf(g, d, acc[1][c]);
+        if constexpr (ACT == SLOPE) acc[2][c] = fmaf(t, z, acc[2][c]);
+      } else {
+        const float vf = v.get(j);
+        acc[0][c] += vf;
+        acc[1][c] = fmaf(vf, d, acc[1][c]);
+        acc[2][c] += g;
+        acc[3][c] = fmaf(g, d, acc[3][c]);
+        acc[4][c] = fmaf(g, vf, acc[4][c]);
+        if constexpr (ACT != KINK) {
+          const float td = t * d;
+          acc[5][c] += t;
+          acc[6][c] += td;
+          acc[7][c] = fmaf(t, vf, acc[7][c]);
+          if constexpr (ACT == SILU) {
+            acc[8][c] = fmaf(td, d, acc[8][c]);
+            acc[9][c] = fmaf(td, vf, acc[9][c]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// Folds acc over the block's positions into chan[k * a.CT + slot] (LDS).  `sh`: scratch of
+// rows: P * CT values, planes: one per wave.  Every thread of the block calls it.
+template <bool ROWS, int V, int K, int NC, class A>
+__device__ __forceinline__ void fold(const Args& a, const Map<ROWS, V>& m, A (&acc)[K][NC], A* sh, A* chan) {
+  const int tid = threadIdx.x, nt = blockDim.x;
+  if constexpr (ROWS) {
+    int Q = 1;                                    // lanes that share a channel's fold
+    while (2 * Q * a.CT <= nt && 2 * Q <= a.P && Q < 64) Q *= 2;
+    for (int k = 0; k < K; ++k) {
+      __syncthreads();
+      if (m.active) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+          if (j >= m.skip0) sh[m.p * a.CT + m.slot + j] = acc[k][j];
+      }
+      __syncthreads();
+      const int q = tid & (Q - 1);
+      for (int c0 = 0; c0 < a.CT; c0 += nt / Q) {
+        const int c = c0 + tid / Q;
+        A s = 0;
+        if (c < a.CT)
+          for (int p = q; p < a.P; p += Q) s += sh[p * a.CT + c];
+        for (int o = Q / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        if (q == 0 && c < a.CT) chan[k * a.CT + c] = s;
+      }
+    }
+    __syncthreads();
+  } else {
+    const int lanes = a.P < 64 ? a.P : 64, nw = a.P / lanes;   // P: a power of two
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      A s = m.active ? acc[k][0] : (A)0;
+      for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+      if (nw == 1) {
+        if (m.p == 0 && m.active) chan[k * a.CT + m.slot] = s;
+      } else if ((tid & 63) == 0) {
+        sh[k * 16 + (tid >> 6)] = s;
+      }
+    }
+    __syncthreads();
+    if (nw > 1) {
+      for (int i = tid; i < K * (nt / a.P); i += nt) {
+        const int k = i / (nt / a.P), s = i % (nt / a.P);
+        if (s < a.CT) {
+          A t = 0;
+          for (int q = 0; q < nw; ++q) t += sh[k * 16 + s * nw + q];
+          chan[k * a.CT + s] = t;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// ------------------------------------------------------------------ group coefficients
+// A channel's terms of the group sums and of the parameter gradients, from its sums over a sample.
+// First sweep (all modes): sums that need no mean.  DBL has a second sweep that needs them.
+struct Group { double mean, r; float mf; double xo; };
+
+__device__ __forceinline__ Group group_of(double mean, double r) {
+  Group q;
+  q.mean = mean;
+  q.r = r;
+  q.mf = (float)mean;
+  q.xo = ((double)q.mf - mean) * r;
+  return q;
+}
+__device__ __forceinline__ double param(const void* p, int dt, int c, double none) {
+  return p ? (double)loadp(p, dt, c) : none;
+}
+
+// BWD: out[2] = w sum g, w sum g xh; terms[3] = gw, gb, gslope
+// DBL: out[4] = sum v, sum v xh, w sum g, w sum g xh
+template <int MODE, int ACT, class S>
+__device__ __forceinline__ void sweep1(const Args& a, const Group& q, int c, S s, double* out, double* terms) {
+  const double w = param(a.w, a.pdt, c, 1.0);
+  if (MODE == BWD) {
+    const double g0 = s(0), gx = q.r * s(1) + q.xo * g0;
+    out[0] += w * g0;
+    out[1] += w * gx;
+    terms[0] = gx;
+    terms[1] = g0;
+    terms[2] = ACT == SLOPE ? s(2) : 0.0;
+  } else {
+    const double v0 = s(0), g0 = s(2);
+    out[0] += v0;
+    out[1] += q.r * s(1) + q.xo * v0;
+    out[2] += w * g0;
+    out[3] += w * (q.r * s(3) + q.xo * g0);
+  }
+}
+// DBL, m[4] the group's means of sweep1: out[3] = terms of N m(e), N m(e xh), N m(u q) beyond the means
+template <int ACT, class S>
+__device__ __forceinline__ void sweep2(const Args& a, const Group& q, int c, S s, const double* m, double* out,
+                                       double* terms) {
+  const double w = param(a.w, a.pdt, c, 1.0), cw = param(a.cw, a.pdt, c, 0.0), cb = param(a.cb, a.pdt, c, 0.0);
+  const double r = q.r, xo = q.xo;
+  const double g0 = s(2), gx = r * s(3) + xo * g0;
+  const double Q = r * (s(4) - m[0] * g0 - m[1] * gx);
+  const double h1 = w * r, h2 = cw - h1 * m[1], h3 = cb - h1 * m[0];   // h = h1 v + h2 xh + h3
+  double T0 = 0.0, T1 = 0.0, sl = 0.0;
+  if (ACT == SILU) {
+    const double k0 = s(5), kx = r * s(6) + xo * k0;
+    const double kxx = r * r * s(8) + 2.0 * r * xo * s(6) + xo * xo * k0;
+    const double kv = s(7), kvx = r * s(9) + xo * kv;
+    T0 = h1 * kv + h2 * kx + h3 * k0;
+    T1 = h1 * kvx + h2 * kxx + h3 * kx;
+  } else if (ACT == SLOPE) {
+    const double cs = param(a.cs, a.pdt, c, 0.0);
+    const double s0 = s(5), sx = r * s(6) + xo * s0;
+    T0 = cs * s0;
+    T1 = cs * sx;
+    sl = h1 * s(7) + h2 * sx + h3 * s0;
+  }
+  out[0] += w * T0 + cw * g0;
+  out[1] += w * T1 + cw * gx;
+  out[2] += w * Q;
+  terms[0] = Q + T1;
+  terms[1] = T0;
+  terms[2] = sl;
+}
+
+// coef[] of a group from its sums.  BWD: {m(u), m(u xh)}; DBL: {m(v), m(v xh), m(u xh), m(e), m(e xh) + m(u q)}
+__device__ __forceinline__ void dbl_coef(const Group& q, const double* m, const double* t, double invN, double* co) {
+  co[0] = m[0];
+  co[1] = m[1];
+  co[2] = m[3];
+  co[3] = -q.r * (m[0] * m[3] + m[2] * m[1]) + t[0] * invN;
+  co[4] = -2.0 * q.r * m[1] * m[3] + t[1] * invN + t[2] * invN;
+}
+
+// The elementwise pass's coefficients of one channel.
+template <int MODE, int ACT>
+struct Lin {
+  Chan<ACT> ch;
+  float B1, C1;                     // BWD: gx = g a + d B1 + C1
+  float H2, H3, G1, V1, D1, K1, cs; // DBL: h = v a + d H2 + H3; g_x = t a + g G1 + v V1 + d D1 + K1
+  __device__ __forceinline__ void set(const Args& g, double mean, double r, const double* co, int c) {
+    ch.set(g, mean, r, c);
+    const double w = param(g.w, g.pdt, c, 1.0), xo = ch.xo;
+    if (MODE == BWD) {
+      B1 = (float)(-r * r * co[1]);
+      C1 = (float)(-r * (co[0] + xo * co[1]));
+    } else if (MODE == DBL) {
+      const double cw = param(g.cw, g.pdt, c, 0.0), cb = param(g.cb, g.pdt, c, 0.0);
+      const double h2 = cw - w * r * co[1];
+      H2 = (float)(h2 * r);
+      H3 = (float)(h2 * xo + cb - w * r * co[0]);
+      G1 = (float)(r * (cw - r * w * co[1]));
+      V1 = (float)(-r * r * co[2]);
+      D1 = (float)(-r * r * co[4]);
+      K1 = (float)(-r * (co[3] + xo * co[4]));
+      cs = ACT == SLOPE ? (float)param(g.cs, g.pdt, c, 0.0) : 0.f;
+    }
+  }
+};
+
+template <int MODE, int ACT, bool ROWS, class T, int V, int NC>
+__device__ __forceinline__ void apply(const Lin<MODE, ACT> (&ln)[NC], const Vec<T, V>& x, const Vec<T, V>& gy,
+                                      const Vec<T, V>& v, Vec<T, V>& o1, Vec<T, V>& o2) {
+  float f1[V], f2[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const Lin<MODE, ACT>& l = ln[ROWS ? j : 0];
+    const float xf = x.get(j);
+    if constexpr (MODE == FWD) {
+      f1[j] = act_fwd<ACT>(l.ch, xf);
+    } else {
+      const float d = xf - l.ch.mf;
+      float g, t, z;
+      act_bwd<ACT>(l.ch, xf, d, gy.get(j), g, t, z);
+      if constexpr (MODE == BWD) {
+        f1[j] = fmaf(g, l.ch.a, fmaf(d, l.B1, l.C1));
+      } else {
+        const float vf = v.get(j);
+        const float h = fmaf(vf, l.ch.a, fmaf(d, l.H2, l.H3));
+        float gg = act_d1<ACT>(l.ch, xf, z) * h, tt = 0.f;
+        if (ACT == SILU) tt = t * h;
+        if (ACT == SLOPE) {
+          tt = l.cs * t;
+          if (!((l.ch.neg ? -xf : xf) >= l.ch.tf)) gg = fmaf(l.cs, z, gg);
+        }
+        f1[j] = gg;
+        f2[j] = fmaf(tt, l.ch.a, fmaf(g, l.G1, fmaf(vf, l.V1, fmaf(d, l.D1, l.K1))));
+      }
+    }
+  }
+  o1.put(f1);
+  if constexpr (MODE == DBL) o2.put(f2);
+}
+
+template <int MODE, int ACT, int NC>
+__device__ __forceinline__ void set_chan(const Args& a, Chan<ACT> (&ch)[NC], const double* stats_b, int c0) {
+  if constexpr (MODE != FWD) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const double* s = stats_b + 2 * ((c0 + j) / a.Cg);
+      ch[j].set(a, s[0], s[1], c0 + j);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ the resident form
+// Block (tile of whole groups, sample): RMAX vectors a thread, held between sums and result.
+template <int MODE, int ACT, bool ROWS, class T, int V, int RMAX, int NTMAX>
+__global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
+  typedef typename AccT<MODE>::type A;
+  constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K;
+  extern __shared__ __align__(16) char lds[];
+  const int tile = blockIdx.x % a.nct;
+  const long b = a.b0 + blockIdx.x / a.nct;
+  const Map<ROWS, V> m(a, b, tile);
+  const int gt = a.CT / a.Cg;                       // groups of a tile (the last may hold fewer)
+  double* gco = reinterpret_cast<double*>(lds);     // [gt][8] (FWD: mean, r)
+  A* chan = reinterpret_cast<A*>(gco + gt * 8);     // [K][CT]
+  A* sh = chan + K * a.CT + (K * a.CT & 1);
+  const T* px = static_cast<const T*>(a.x);
+  const T* pg = static_cast<const T*>(a.gy);
+  const T* pv = static_cast<const T*>(a.v);
+
+  Vec<T, V> x[RMAX], gy[MODE >= BWD ? RMAX : 1], v[MODE == DBL ? RMAX : 1];
+#pragma unroll
+  for (int k = 0; k < RMAX; ++k) {
+    const int i = m.p + k * a.P;
+    if (m.active && i < m.npos) {
+      int skip;
+      const long at = m.at(i, skip);
+      x[k] = load<T, V>(px + at);
+      if constexpr (MODE >= BWD) gy[k] = load<T, V>(pg + at);
+      if constexpr (MODE == DBL) v[k] = load<T, V>(pv + at);
+      if (MODE == FWD) x[k].zero_front(skip);
+      if constexpr (MODE >= BWD) gy[k].zero_front(skip);
+      if constexpr (MODE == DBL) v[k].zero_front(skip);
+    } else {
+      x[k].zero_front(V);
+      if constexpr (MODE >= BWD) gy[k].zero_front(V);
+      if constexpr (MODE == DBL) v[k].zero_front(V);
+    }
+  }
+  Chan<ACT> ch[NC];
+  set_chan<MODE>(a, ch, a.stats + 2 * b * a.G, m.ch);
+  A acc[K][NC];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[k][j] = 0;
+#pragma unroll
+  for (int k = 0; k < RMAX; ++k)
+    if (k == 0 || k * a.P < m.npos)
+      accumulate<MODE, ACT, ROWS, T, V, NC>(acc, ch, x[k], gy[MODE >= BWD ? k : 0], v[MODE == DBL ? k : 0]);
+#pragma unroll
+  for (int k = 0; k < RMAX; ++k) {
+    x[k].pin();
+    if constexpr (MODE >= BWD) gy[k].pin();
+    if constexpr (MODE == DBL) v[k].pin();
+  }
+  fold<ROWS, V, K, NC>(a, m, acc, sh, chan);
+
+  // groups: one wave each
+  const int lane = threadIdx.x & 63, nw = blockDim.x >> 6;
+  const int c0 = tile * a.CT, g0 = c0 / a.Cg, ng = min(gt, a.G - g0);
+  const double invN = 1.0 / ((double)a.L * a.Cg);
+  for (int gi = threadIdx.x >> 6; gi < ng; gi += nw) {
+    const int cg = gi * a.Cg;
+    double* st = a.stats + 2 * (b * a.G + g0 + gi);
+    if constexpr (MODE == FWD) {
+      double s = 0, q = 0;
+      for (int c = lane; c < a.Cg; c += 64) {
+        s += chan[cg + c];
+        q += chan[a.CT + cg + c];
+      }
+      s = wave_sum(s);
+      q = wave_sum(q);
+      const double mean = s * invN, var = fmax(q * invN - mean * mean, 0.0);
+      const double nan = s - s + (q - q);            // fmax drops a NaN: put it back
+      const double r = 1.0 / sqrt(var + nan + (double)a.eps);
+      if (lane == 0) {
+        gco[gi * 8] = mean;
+        gco[gi * 8 + 1] = r;
+        st[0] = mean;
+        st[1] = r;
+      }
+    } else {
+      const Group q = group_of(st[0], st[1]);
+      const int cc = c0 + cg;
+      double m1[4] = {0, 0, 0, 0};
+      for (int c = lane; c < a.Cg; c += 64) {
+        double terms[3];
+        sweep1<MODE, ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * a.CT + cg + c]; }, m1, terms);
+        if (MODE == BWD && a.par)
+          for (int k = 0; k < Sums<BWD, ACT>::K; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
+      }
+      for (int k = 0; k < (MODE == BWD ? 2 : 4); ++k) m1[k] = wave_sum(m1[k]) * invN;
+      if (MODE == BWD) {
+        if (lane == 0) {
+          gco[gi * 8] = m1[0];
+          gco[gi * 8 + 1] = m1[1];
+        }
+      } else {
+        double m2[3] = {0, 0, 0};
+        for (int c = lane; c < a.Cg; c += 64) {
+          double terms[3];
+          sweep2<ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * a.CT + cg + c]; }, m1, m2, terms);
+          if (a.par)
+            for (int k = 0; k < 3; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
+        }
+        for (int k = 0; k < 3; ++k) m2[k] = wave_sum(m2[k]);
+        if (lane == 0) dbl_coef(q, m1, m2, invN, gco + gi * 8);
+      }
+    }
+  }
+  __syncthreads();
+  if (!m.active) return;
+  Lin<MODE, ACT> ln[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int c = m.ch + j, gi = c / a.Cg - g0;
+    if (gi >= 0 && gi < ng) {                        // (a moved-back vector's front lies in another tile)
+      const double* st = MODE == FWD ? gco + gi * 8 : a.stats + 2 * (b * a.G + g0 + gi);
+      ln[j].set(a, st[0], st[1], gco + gi * 8, c);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < RMAX; ++k) {
+    const int i = m.p + k * a.P;
+    if (i < m.npos) {
+      int skip;
+      const long at = m.at(i, skip);
+      Vec<T, V> o1, o2;
+      apply<MODE, ACT, ROWS, T, V, NC>(ln, x[k], gy[MODE >= BWD ? k : 0], v[MODE == DBL ? k : 0], o1, o2);
+      if (MODE != BWD || a.o1) store(static_cast<T*>(a.o1) + at, o1, skip);
+      if constexpr (MODE == DBL)
+        if (a.o2) store(static_cast<T*>(a.o2) + at, o2, skip);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ the split form
+constexpr int kNT = 512;
+
+// blockIdx.x = (sample, tile, chunk), chunk fastest
+template <int MODE, int ACT, bool ROWS, class T, int V>
+__global__ __launch_bounds__(kNT) void sums_kernel(Args a) {
+  typedef typename AccT<MODE>::type A;
+  constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K, U = 4;
+  extern __shared__ __align__(16) char lds[];
+  const int s = blockIdx.x % a.S, tile = blockIdx.x / a.S % a.nct;
+  const int bi = blockIdx.x / a.S / a.nct;
+  const long b = a.b0 + bi;
+  const Map<ROWS, V> m(a, b, tile);
+  A* chan = reinterpret_cast<A*>(lds);
+  A* sh = chan + K * a.CT + (K * a.CT & 1);
+  const T* px = static_cast<const T*>(a.x);
+  const T* pg = static_cast<const T*>(a.gy);
+  const T* pv = static_cast<const T*>(a.v);
+  Chan<ACT> ch[NC];
+  set_chan<MODE>(a, ch, a.stats + 2 * b * a.G, m.ch);
+  A acc[K][NC];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[k][j] = 0;
+  const int hi = (int)min((long)m.npos, (long)(s + 1) * a.per);
+  if (m.active) {
+    for (int i0 = s * a.per + m.p; i0 < hi; i0 += U * a.P) {
+      Vec<T, V> x[U], gy[MODE >= BWD ? U : 1], v[MODE == DBL ? U : 1];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * a.P;
+        int skip = V;
+        if (i < hi) {
+          const long at = m.at(i, skip);
+          x[u] = load<T, V>(px + at);
+          if constexpr (MODE >= BWD) gy[u] = load<T, V>(pg + at);
+          if constexpr (MODE == DBL) v[u] = load<T, V>(pv + at);
+        }
+        if (MODE == FWD || skip == V) x[u].zero_front(skip);
+        if constexpr (MODE >= BWD) gy[u].zero_front(skip);
+        if constexpr (MODE == DBL) v[u].zero_front(skip);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        accumulate<MODE, ACT, ROWS, T, V, NC>(acc, ch, x[u], gy[MODE >= BWD ? u : 0], v[MODE == DBL ? u : 0]);
+    }
+  }
+  fold<ROWS, V, K, NC>(a, m, acc, sh, chan);
+  const int c0 = tile * a.CT, wid = min(a.CT, a.C - c0);
+  A* part = reinterpret_cast<A*>(a.part) + ((long)bi * a.S + s) * K * a.C;
+  for (int i = threadIdx.x; i < K * wid; i += blockDim.x)
+    part[(long)(i / wid) * a.C + c0 + i % wid] = chan[i / wid * a.CT + i % wid];
+}
+
+// Block (sample, group): the chunks' sums folded, in double and in one order; the group's coefficients.
+template <int MODE, int ACT>
+__global__ __launch_bounds__(256) void group_kernel(Args a) {
+  typedef typename AccT<MODE>::type A;
+  constexpr int K = Sums<MODE, ACT>::K;
+  __shared__ double red[4][4], sh[256];
+  extern __shared__ __align__(16) char lds[];
+  double* chan = reinterpret_cast<double*>(lds);      // [K][min(Cg, 256)]: a pass of channels
+  const int gi = blockIdx.x % a.G, bi = blockIdx.x / a.G;
+  const long b = a.b0 + bi;
+  const int tid = threadIdx.x;
+  int cw = 1;
+  while (cw < a.Cg && cw < 256) cw *= 2;
+  const int sw = 256 / cw, ci = tid % cw, si = tid / cw;
+  const A* part = reinterpret_cast<const A*>(a.part) + (long)bi * a.S * K * a.C + gi * a.Cg;
+  double* st = a.stats + 2 * (b * a.G + gi);
+  Group q = {0, 0, 0, 0};
+  if (MODE != FWD) q = group_of(st[0], st[1]);
+  const double invN = 1.0 / ((double)a.L * a.Cg);
+  double m1[4] = {0, 0, 0, 0}, m2[3] = {0, 0, 0};
+  for (int sweep = 0; sweep < (MODE == DBL ? 2 : 1); ++sweep) {
+    for (int cb = 0; cb < a.Cg; cb += cw) {
+      const int c = cb + ci;
+      if (sweep == 0 || a.Cg > cw) {
+        for (int k = 0; k < K; ++k) {
+          double t = 0;
+          if (c < a.Cg)
+            for (int s = si; s < a.S; s += sw) t += (double)part[((long)s * K + k) * a.C + c];
+          __syncthreads();
+          sh[tid] = t;
+          __syncthreads();
+          if (si == 0) {
+            for (int i = 1; i < sw; ++i) t += sh[i * cw + ci];
+            chan[k * cw + ci] = t;
+          }
+        }
+      }
+      if (si == 0 && c < a.Cg) {                      // (reads back what this thread wrote)
+        const int cc = gi * a.Cg + c;
+        auto get = [&](int k) { return chan[k * cw + ci]; };
+        double terms[3] = {0, 0, 0};
+        if constexpr (MODE == FWD) {
+          m1[0] += get(0);
+          m1[1] += get(1);
+        } else if (sweep == 0) {
+          sweep1<MODE, ACT>(a, q, cc, get, m1, terms);
+        } else {
+          sweep2<ACT>(a, q, cc, get, m1, m2, terms);
+        }
+        if (MODE != FWD && a.par && (MODE == BWD || sweep == 1))
+          for (int k = 0; k < (MODE == BWD ? Sums<BWD, ACT>::K : 3); ++k)
+            a.par[(k * a.B + b) * a.C + cc] = (float)terms[k];
+      }
+    }
+    double* mm = sweep == 0 ? m1 : m2;
+    const int n = sweep == 0 ? 4 : 3;
+    for (int k = 0; k < n; ++k) {
+      const double t = wave_sum(mm[k]);
+      if ((tid & 63) == 0) red[k][tid >> 6] = t;
+    }
+    __syncthreads();
+    for (int k = 0; k < n; ++k) mm[k] = (red[k][0] + red[k][1]) + (red[k][2] + red[k][3]);
+    __syncthreads();
+    if (MODE != FWD && sweep == 0)
+      for (int k = 0; k < 4; ++k) m1[k] *= invN;
+  }
+  if (tid != 0) return;
+  double* co = a.coef + 8 * (b * a.G + gi);
+  if constexpr (MODE == FWD) {
+    const double mean = m1[0] * invN, var = fmax(m1[1] * invN - mean * mean, 0.0);
+    const double nan = m1[0] - m1[0] + (m1[1] - m1[1]);
+    st[0] = mean;
+    st[1] = 1.0 / sqrt(var + nan + (double)a.eps);
+  } else if constexpr (MODE == BWD) {
+    co[0] = m1[0];
+    co[1] = m1[1];
+  } else {
+    dbl_coef(q, m1, m2, invN, co);
+  }
+}
+
+template <int MODE, int ACT, bool ROWS, class T, int V>
+__global__ __launch_bounds__(kNT) void apply_kernel(Args a) {
+  constexpr int NC = ROWS ? V : 1, U = 2;
+  const int s = blockIdx.x % a.S, tile = blockIdx.x / a.S % a.nct;
+  const long b = a.b0 + blockIdx.x / a.S / a.nct;
+  const Map<ROWS, V> m(a, b, tile);
+  if (!m.active) return;
+  const T* px = static_cast<const T*>(a.x);
+  const T* pg = static_cast<const T*>(a.gy);
+  const T* pv = static_cast<const T*>(a.v);
+  Lin<MODE, ACT> ln[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const long g = b * a.G + (m.ch + j) / a.Cg;
+    ln[j].set(a, a.stats[2 * g], a.stats[2 * g + 1], a.coef + 8 * g, m.ch + j);
+  }
+  const int hi = (int)min((long)m.npos, (long)(s + 1) * a.per);
+  for (int i0 = s * a.per + m.p; i0 < hi; i0 += U * a.P) {
+    Vec<T, V> x[U], gy[MODE >= BWD ? U : 1], v[MODE == DBL ? U : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * a.P;
+      if (i < hi) {
+        int skip;
+        const long at = m.at(i, skip);
+        x[u] = load<T, V>(px + at);
+        if constexpr (MODE >= BWD) gy[u] = load<T, V>(pg + at);
+        if constexpr (MODE == DBL) v[u] = load<T, V>(pv + at);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * a.P;
+      if (i < hi) {
+        int skip;
+        const long at = m.at(i, skip);
+        Vec<T, V> o1, o2;
+        apply<MODE, ACT, ROWS, T, V, NC>(ln, x[u], gy[MODE >= BWD ? u : 0], v[MODE == DBL ? u : 0], o1, o2);
+        if (MODE != BWD || a.o1) store(static_cast<T*>(a.o1) + at, o1, skip);
+        if constexpr (MODE == DBL)
+          if (a.o2) store(static_cast<T*>(a.o2) + at, o2, skip);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ launches
+// Threads of a resident block and the vectors of each input that a thread can hold: what fits
+// 256 registers a thread (512 threads) or 128 (1024; one input).
+constexpr int resident_threads(int mode, bool rows) { return rows || mode != FWD ? 512 : 1024; }
+constexpr int resident_vectors(int mode) { return mode == DBL ? 8 : 16; }
+
+// How one call runs (group_norm.hip makes it from sizes and type alone).
+struct Plan {
+  int mode, act;
+  bool rows, resident;
+  int V, rmax, nt;
+  size_t lds, group_lds;
+  int slice;              // samples per slice
+};
+
+template <int MODE, int ACT, bool ROWS, class T, int V, int RMAX>
+int launch_resident(const Plan& p, const Args& a, long nb, hipStream_t st) {
+  constexpr int NTMAX = resident_threads(MODE, ROWS);
+  hipLaunchKernelGGL((resident_kernel<MODE, ACT, ROWS, T, V, RMAX, NTMAX>), dim3((unsigned)(nb * a.nct)), dim3(p.nt),
+                     p.lds, st, a);
+  return hipGetLastError() == hipSuccess ? GANAMD_OK : GANAMD_ELAUNCH;
+}
+
+template <int MODE, int ACT, bool ROWS, class T, int V>
+int launch_v(const Plan& p, const Args& a, long nb, hipStream_t st) {
+  if (p.resident) {
+    constexpr int MOST = resident_vectors(MODE);
+    if (p.rmax <= 2) return launch_resident<MODE, ACT, ROWS, T, V, 2>(p, a, nb, st);
+    if (p.rmax <= MOST / 2) return launch_resident<MODE, ACT, ROWS, T, V, MOST / 2>(p, a, nb, st);
+    return launch_resident<MODE, ACT, ROWS, T, V, MOST>(p, a, nb, st);
+  }
+  const dim3 grid((unsigned)(nb * a.nct * a.S));
+  hipLaunchKernelGGL((sums_kernel<MODE, ACT, ROWS, T, V>), grid, dim3(p.nt), p.lds, st, a);
+  hipLaunchKernelGGL((group_kernel<MODE, ACT>), dim3((unsigned)(nb * a.G)), dim3(256), p.group_lds, st, a);
+  if (MODE != BWD || a.o1) hipLaunchKernelGGL((apply_kernel<MODE, ACT, ROWS, T, V>), grid, dim3(p.nt), 0, st, a);
+  return hipGetLastError() == hipSuccess ? GANAMD_OK : GANAMD_ELAUNCH;
+}
+
+// vector width of an element type: 16 bytes; 4 elements where a thread carries the sums and
+// coefficients of each of its channels (rows, backward), 1 where rows / planes are shorter
+constexpr int vec_width(int mode, bool rows, int size) { return rows && mode != FWD ? 4 : 16 / size; }
+
+template <int MODE, int ACT, class T>
+int launch_t(const Plan& p, const Args& a, long nb, hipStream_t st) {
+  constexpr int VR = vec_width(MODE, true, sizeof(T)), VP = vec_width(MODE, false, sizeof(T));
+  if (p.rows) return p.V == 1 ? launch_v<MODE, ACT, true, T, 1>(p, a, nb, st) : launch_v<MODE, ACT, true, T, VR>(p, a, nb, st);
+  return p.V == 1 ? launch_v<MODE, ACT, false, T, 1>(p, a, nb, st) : launch_v<MODE, ACT, false, T, VP>(p, a, nb, st);
+}
+
+template <class T>
+int launch(const Plan& p, const Args& a, long nb, hipStream_t st) {
+  if (p.mode == FWD)
+    return p.act == SILU ? launch_t<FWD, SILU, T>(p, a, nb, st) : launch_t<FWD, KINK, T>(p, a, nb, st);
+  if (p.mode == BWD)
+    return p.act == SILU ? launch_t<BWD, SILU, T>(p, a, nb, st)
+         : p.act == KINK ? launch_t<BWD, KINK, T>(p, a, nb, st) : launch_t<BWD, SLOPE, T>(p, a, nb, st);
+  return p.act == SILU ? launch_t<DBL, SILU, T>(p, a, nb, st)
+       : p.act == KINK ? launch_t<DBL, KINK, T>(p, a, nb, st) : launch_t<DBL, SLOPE, T>(p, a, nb, st);
+}
+
+// one translation unit per element type (compiled in parallel)
+int launch_f32(const Plan& p, const Args& a, long nb, hipStream_t st);
+int launch_bf16(const Plan& p, const Args& a, long nb, hipStream_t st);
+int launch_f16(const Plan& p, const Args& a, long nb, hipStream_t st);
+
+}  // namespace gn

@@ -1,0 +1,270 @@
+// Group norm with its activation: plans, workspaces and the C entry points (kernels: group_norm.h).
+#include "group_norm.h"
+
+#include <algorithm>
+
+namespace {
+
+using gn::Args;
+using gn::Plan;
+
+inline long up_to(long a, long b) { return (a + b - 1) / b; }
+inline long pow2_at_least(long n) {
+  long p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+
+bool valid(const ganamd_norm_desc* d) {
+  return d && d->B > 0 && d->C > 0 && d->L > 0 && d->L <= (1L << 30) && d->G > 0 && d->C % d->G == 0 &&
+         d->C <= (1 << 24) && (d->layout == GANAMD_NORM_ROWS || d->layout == GANAMD_NORM_PLANES) &&
+         d->dtype >= GANAMD_F32 && d->dtype <= GANAMD_F16 && d->param_dtype >= GANAMD_F32 &&
+         d->param_dtype <= GANAMD_F16 && d->act >= GANAMD_NORM_NONE && d->act <= GANAMD_NORM_PRELU && d->eps > 0.f;
+}
+
+int esize(int dt) { return dt == GANAMD_F32 ? 4 : 2; }
+
+struct Full {
+  Plan p;
+  Args a;                          // the sizes; no pointers
+  size_t part, coef, par, fold, total;   // workspace offsets and size
+};
+
+constexpr int kFoldB = 512;        // samples a parameter-gradient block folds
+
+// Which kernels a call takes and how its work is cut, from the sizes and the type alone.
+bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
+  if (!valid(d)) return false;
+  Plan& p = f.p;
+  Args& a = f.a;
+  a = Args{};
+  const int esz = esize(d->dtype);
+  const int C = d->C, G = d->G, Cg = C / G;
+  const long L = d->L, B = d->B;
+  p.mode = mode;
+  p.rows = d->layout == GANAMD_NORM_ROWS;
+  p.act = d->act == GANAMD_NORM_SILU ? gn::SILU
+        : d->act == GANAMD_NORM_PRELU && mode != gn::FWD ? gn::SLOPE : gn::KINK;
+  p.V = gn::vec_width(mode, p.rows, esz);
+  if ((p.rows ? (long)C : L) < p.V) p.V = 1;
+  const int K = mode == gn::FWD ? 2 : mode == gn::BWD ? (p.act == gn::SLOPE ? 3 : 2)
+              : (p.act == gn::SILU ? 10 : p.act == gn::SLOPE ? 8 : 5);
+  const size_t asz = mode == gn::FWD ? 8 : 4;
+  const int rcap = gn::resident_vectors(mode), most = gn::resident_threads(mode, p.rows);
+  a.L = L; a.B = B; a.C = C; a.G = G; a.Cg = Cg; a.eps = d->eps; a.pdt = d->param_dtype;
+  a.cslope = d->act == GANAMD_NORM_LEAKY ? d->slope : 1.f;
+  p.resident = false;
+  p.slice = (int)B;
+  const long nv = up_to(L, p.V);
+  if (p.rows) {
+    // a tile of whole groups, at least a cache line wide
+    long gt = 1;
+    while (gt < G && (gt * Cg * esz < 128 || gt * Cg < p.V)) ++gt;
+    for (long t = gt; t <= G && t < gt + p.V; ++t)
+      if (t * Cg % p.V == 0) { gt = t; break; }
+    if (gt * Cg < p.V) gt = G;
+    const long CT = gt * Cg, TX = up_to(CT, p.V);
+    if (TX <= most) {
+      const long P = std::min<long>(most / TX, L), R = up_to(L, P), nct = up_to(G, gt);
+      if (R <= rcap && (R <= 2 || B * nct >= 96)) {
+        p.resident = true;
+        a.TX = (int)TX; a.P = (int)P; a.CT = (int)CT; a.nct = (int)nct; p.rmax = (int)R;
+        p.nt = (int)up_to(TX * P, 64) * 64;
+      }
+    }
+  } else if (Cg <= most) {
+    long P = std::min(pow2_at_least(nv), pow2_at_least(most / Cg + 1) / 2), gt = 1;
+    while (gt < G && (gt + 1) * Cg * P <= 256 && B * up_to(G, gt + 1) >= 512) ++gt;
+    const long R = up_to(nv, P), nct = up_to(G, gt);
+    if (R <= rcap && (R <= 2 || B * nct >= 96)) {
+      p.resident = true;
+      a.TX = (int)(gt * Cg); a.P = (int)P; a.CT = (int)(gt * Cg); a.nct = (int)nct; p.rmax = (int)R;
+      p.nt = (int)up_to(a.TX * P, 64) * 64;
+    }
+  }
+  if (p.resident) {
+    a.S = 1;
+    a.per = 0;
+    const size_t sh = p.rows ? (size_t)a.P * a.CT : (size_t)K * 16;
+    p.lds = (size_t)(a.CT / Cg) * 64 + asz * ((size_t)K * a.CT + 1 + sh);
+    if (p.lds > 64 * 1024) p.resident = false;
+  }
+  if (!p.resident) {
+    long npos;
+    if (p.rows) {
+      const long all = up_to(C, p.V);
+      // (a tile's channels: their sums, K each, and the fold's scratch share 64 KB)
+      a.nct = (int)std::max(up_to(all, gn::kNT), up_to(all * p.V * K * (long)asz, 24 * 1024));
+      a.TX = (int)up_to(all, a.nct);
+      a.CT = a.TX * p.V;
+      a.nct = (int)up_to(C, a.CT);
+      a.P = (int)std::min<long>(gn::kNT / a.TX, L);
+      p.nt = (int)up_to((long)a.TX * a.P, 64) * 64;
+      npos = L;
+    } else {
+      a.P = (int)std::min<long>(gn::kNT, pow2_at_least(nv));
+      a.CT = a.TX = (int)std::min<long>(gn::kNT / a.P, C);
+      a.nct = (int)up_to(C, a.CT);
+      p.nt = (int)up_to((long)a.TX * a.P, 64) * 64;
+      npos = nv;
+    }
+    // four blocks of eight waves a CU, but four vectors a thread at least, and at most 128 values of
+    // a channel in one thread's fp32 sums
+    long S = std::max<long>(1, std::min(up_to(1024, B * a.nct), up_to(npos, 4L * a.P)));
+    S = std::max(S, up_to(npos, (p.rows ? 128L : 128L / p.V) * a.P));
+    a.per = (int)(up_to(up_to(npos, S), a.P) * a.P);
+    a.S = (int)up_to(npos, a.per);
+    const size_t sh = p.rows ? (size_t)a.P * a.CT : (size_t)K * 16;
+    p.lds = asz * ((size_t)K * a.CT + 1 + sh);
+  }
+  p.group_lds = 8 * (size_t)K * std::min<long>(256, pow2_at_least(Cg));
+  if (B * a.nct * a.S >= (1L << 31) || B * G >= (1L << 31) || p.lds > 64 * 1024) return false;
+  // workspace
+  size_t at = 0;
+  auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
+  f.part = p.resident ? 0 : take(asz * (size_t)K * C * a.S * p.slice);
+  f.coef = p.resident || mode == gn::FWD ? 0 : take(64 * (size_t)B * G);
+  f.par = mode == gn::FWD ? 0 : take(4 * 3 * (size_t)B * C);
+  f.fold = mode == gn::FWD || B <= kFoldB ? 0 : take(4 * 3 * (size_t)up_to(B, kFoldB) * C);
+  f.total = at;
+  return true;
+}
+
+__device__ __forceinline__ void put(void* out, int dt, long i, double v, int accumulate) {
+  if (dt == GANAMD_F32) {
+    float* o = static_cast<float*>(out) + i;
+    *o = accumulate ? *o + (float)v : (float)v;
+  } else if (dt == GANAMD_BF16) {
+    gn::bf16* o = static_cast<gn::bf16*>(out) + i;
+    *o = gn::down<gn::bf16>((accumulate ? gn::up(*o) : 0.f) + (float)v);
+  } else {
+    gn::f16* o = static_cast<gn::f16*>(out) + i;
+    *o = gn::down<gn::f16>((accumulate ? gn::up(*o) : 0.f) + (float)v);
+  }
+}
+
+// Sums in[k][b][c] over chunks of `n` samples, in double and one order; the last stage writes the
+// gradients, an earlier one in's successor mid[k][chunk][c].  Block: 64 channels x 16 samples.
+__global__ __launch_bounds__(1024) void param_kernel(const float* __restrict__ in, long B, int C, int n, float* mid,
+                                                     void* g0, void* g1, void* g2, int dt, int accumulate) {
+  __shared__ double sh[16][64];
+  const int k = blockIdx.y, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const long chunk = blockIdx.z, c = blockIdx.x * 64L + x;
+  void* out = k == 0 ? g0 : k == 1 ? g1 : g2;
+  if (!mid && !out) return;
+  const long hi = min(B, (chunk + 1) * n);
+  double t = 0;
+  if (c < C) {
+#pragma unroll 4
+    for (long b = chunk * n + y; b < hi; b += 16) t += (double)in[(k * B + b) * C + c];
+  }
+  sh[y][x] = t;
+  __syncthreads();
+  if (y != 0 || c >= C) return;
+  for (int i = 1; i < 16; ++i) t += sh[i][x];
+  if (mid)
+    mid[((long)k * gridDim.z + chunk) * C + c] = (float)t;
+  else
+    put(out, dt, c, t, accumulate);
+}
+
+int fold_params(const Full& f, char* ws, int K, void* gw, void* gb, void* gs, int dt, int accumulate, hipStream_t st) {
+  if (!gw && !gb && !gs) return GANAMD_OK;
+  const float* in = reinterpret_cast<const float*>(ws + f.par);
+  long B = f.a.B;
+  const int C = f.a.C;
+  const unsigned gx = (unsigned)up_to(C, 64);
+  if (B > kFoldB) {
+    float* mid = reinterpret_cast<float*>(ws + f.fold);
+    const long nc = up_to(B, kFoldB);
+    if (nc > 65535) return GANAMD_EINVAL;
+    hipLaunchKernelGGL(param_kernel, dim3(gx, K, (unsigned)nc), dim3(1024), 0, st, in, B, C, kFoldB, mid, gw, gb, gs, dt, 0);
+    in = mid;
+    B = nc;
+  }
+  hipLaunchKernelGGL(param_kernel, dim3(gx, K, 1), dim3(1024), 0, st, in, B, C, (int)B, (float*)nullptr, gw, gb, gs,
+                     dt, accumulate);
+  return hipGetLastError() == hipSuccess ? GANAMD_OK : GANAMD_ELAUNCH;
+}
+
+int run(const ganamd_norm_desc* d, const Full& f, Args a, char* ws, hipStream_t st) {
+  a.part = reinterpret_cast<float*>(ws + f.part);
+  a.coef = reinterpret_cast<double*>(ws + f.coef);
+  for (long b0 = 0; b0 < f.a.B; b0 += f.p.slice) {
+    a.b0 = (int)b0;
+    const long nb = std::min<long>(f.p.slice, f.a.B - b0);
+    const int rc = d->dtype == GANAMD_F32 ? gn::launch_f32(f.p, a, nb, st)
+                 : d->dtype == GANAMD_BF16 ? gn::launch_bf16(f.p, a, nb, st) : gn::launch_f16(f.p, a, nb, st);
+    if (rc != GANAMD_OK) return rc;
+  }
+  return GANAMD_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ganamd_group_norm_workspace(const ganamd_norm_desc* d, int op, size_t* bytes) {
+  Full f;
+  if (!bytes || op < gn::FWD || op > gn::DBL || !make_plan(d, op, f)) return GANAMD_EINVAL;
+  *bytes = f.total;
+  return GANAMD_OK;
+}
+
+int ganamd_group_norm_plan_info(const ganamd_norm_desc* d, int op, int* info) {
+  Full f;
+  if (!info || op < gn::FWD || op > gn::DBL || !make_plan(d, op, f)) return GANAMD_EINVAL;
+  const int v[10] = {f.p.resident, f.p.V, f.p.nt, f.a.TX, f.a.P, f.a.CT, f.a.nct, f.a.S, f.a.per, f.p.slice};
+  for (int i = 0; i < 10; ++i) info[i] = v[i];
+  return GANAMD_OK;
+}
+
+int ganamd_group_norm_fwd(const ganamd_norm_desc* d, const void* x, const void* w, const void* b, const void* slope,
+                          void* y, double* stats, void* workspace, size_t workspace_bytes, hipStream_t st) {
+  Full f;
+  if (!make_plan(d, gn::FWD, f) || !x || !y || !stats || (d->act == GANAMD_NORM_PRELU && !slope) ||
+      workspace_bytes < f.total || (f.total && !workspace))
+    return GANAMD_EINVAL;
+  Args a = f.a;
+  a.x = x; a.w = w; a.b = b; a.slope = d->act == GANAMD_NORM_PRELU ? slope : nullptr;
+  a.o1 = y; a.stats = stats;
+  return run(d, f, a, static_cast<char*>(workspace), st);
+}
+
+int ganamd_group_norm_bwd(const ganamd_norm_desc* d, const void* gy, const void* x, const void* w, const void* b,
+                          const void* slope, const double* stats, void* gx, void* gw, void* gb, void* gslope,
+                          int accumulate, void* workspace, size_t workspace_bytes, hipStream_t st) {
+  Full f;
+  if (!make_plan(d, gn::BWD, f) || !gy || !x || !stats || (d->act == GANAMD_NORM_PRELU && !slope) ||
+      (gslope && d->act != GANAMD_NORM_PRELU) || workspace_bytes < f.total || (f.total && !workspace))
+    return GANAMD_EINVAL;
+  if (!gx && !gw && !gb && !gslope) return GANAMD_OK;
+  char* ws = static_cast<char*>(workspace);
+  Args a = f.a;
+  a.x = x; a.gy = gy; a.w = w; a.b = b; a.slope = d->act == GANAMD_NORM_PRELU ? slope : nullptr;
+  a.o1 = gx; a.stats = const_cast<double*>(stats);
+  a.par = gw || gb || gslope ? reinterpret_cast<float*>(ws + f.par) : nullptr;
+  const int rc = run(d, f, a, ws, st);
+  return rc != GANAMD_OK ? rc : fold_params(f, ws, gslope ? 3 : 2, gw, gb, gslope, d->param_dtype, accumulate, st);
+}
+
+int ganamd_group_norm_bwd_bwd(const ganamd_norm_desc* d, const void* ggx, const void* ggw, const void* ggb,
+                              const void* ggslope, const void* gy, const void* x, const void* w, const void* b,
+                              const void* slope, const double* stats, void* g_gy, void* g_x, void* g_w, void* g_b,
+                              void* g_slope, int accumulate, void* workspace, size_t workspace_bytes, hipStream_t st) {
+  Full f;
+  if (!make_plan(d, gn::DBL, f) || !ggx || !gy || !x || !stats || !g_gy || !g_x ||
+      (d->act == GANAMD_NORM_PRELU && !slope) || ((g_slope || ggslope) && d->act != GANAMD_NORM_PRELU) ||
+      workspace_bytes < f.total || (f.total && !workspace))
+    return GANAMD_EINVAL;
+  char* ws = static_cast<char*>(workspace);
+  Args a = f.a;
+  a.x = x; a.gy = gy; a.v = ggx; a.w = w; a.b = b; a.slope = d->act == GANAMD_NORM_PRELU ? slope : nullptr;
+  a.cw = ggw; a.cb = ggb; a.cs = ggslope;
+  a.o1 = g_gy; a.o2 = g_x; a.stats = const_cast<double*>(stats);
+  a.par = g_w || g_b || g_slope ? reinterpret_cast<float*>(ws + f.par) : nullptr;
+  const int rc = run(d, f, a, ws, st);
+  return rc != GANAMD_OK ? rc : fold_params(f, ws, g_slope ? 3 : 2, g_w, g_b, g_slope, d->param_dtype, accumulate, st);
+}
+
+}  // extern "C"

@@ -16,8 +16,8 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import LIB, check, iptr, ptr, stream
-from .ops import PackRegistry, invalidate_packed
+from ._lib import LIB, GanAmdError, check, iptr, ptr, stream
+from .ops import PackRegistry, clipped_adamw_, invalidate_packed
 
 
 def _never_gets_grad(owner_cls: str, pname: str) -> bool:
@@ -63,15 +63,25 @@ class FlatParams:
 
 
 class FusedAdamW:
-    """Drop-in for ``torch.optim.AdamW(module.parameters(), lr, betas)`` over FlatParams."""
+    """Drop-in for ``torch.optim.AdamW(module.parameters(), lr, betas)`` over FlatParams.
 
-    def __init__(self, module: torch.nn.Module, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    ``max_grad_norm``: every step clips the gradient to this global norm first
+    (``torch.nn.utils.clip_grad_norm_`` before ``step()``, fused into it: the gradient buffer stays
+    unscaled); ``grad_norm`` then holds the last step's norm before the clip, on the device.  Under
+    data parallelism the norm is the averaged gradient's (``dist.attach_grad_sync`` reduces first)."""
+
+    def __init__(self, module: torch.nn.Module, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 max_grad_norm=None):
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0:
+            raise GanAmdError(f"FusedAdamW: max_grad_norm {max_grad_norm}")
         self.flat = FlatParams(module)
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
         dev = self.flat.data.device
         self.exp_avg = torch.zeros(self.flat.n_train, device=dev, dtype=torch.float32)
         self.exp_avg_sq = torch.zeros_like(self.exp_avg)
         self.step_count = torch.zeros(1, device=dev, dtype=torch.int32)
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = torch.zeros((), device=dev, dtype=torch.float32)
 
     def zero_grad(self, set_to_none: bool = False):
         self.flat.zero_grad()
@@ -93,8 +103,12 @@ class FusedAdamW:
     @torch.no_grad()
     def step(self):
         f = self.flat
-        check(LIB.ganamd_adamw(ptr(f.data), ptr(f.grad), ptr(self.exp_avg), ptr(self.exp_avg_sq), f.n_train,
-                               iptr(self.step_count), float(self.lr), float(self.betas[0]), float(self.betas[1]),
-                               float(self.eps), float(self.weight_decay), stream()), "adamw")
+        if self.max_grad_norm is not None:
+            clipped_adamw_(f.data[:f.n_train], f.grad, self.exp_avg, self.exp_avg_sq, self.step_count, self.lr,
+                           self.betas, self.eps, self.weight_decay, self.max_grad_norm, norm=self.grad_norm)
+        else:
+            check(LIB.ganamd_adamw(ptr(f.data), ptr(f.grad), ptr(self.exp_avg), ptr(self.exp_avg_sq), f.n_train,
+                                   iptr(self.step_count), float(self.lr), float(self.betas[0]), float(self.betas[1]),
+                                   float(self.eps), float(self.weight_decay), stream()), "adamw")
         f.epoch += 1   # packed conv weights of these parameters (ops.PackCache) are stale now ...
         f.packs.repack()   # ... until this one launch refreshes every registered copy

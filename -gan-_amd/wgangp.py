@@ -43,8 +43,11 @@ def _frozen(module):
 
 
 class Train(CheckpointMixin):
+    """``max_grad_norm``: both optimizers clip their gradient to this global norm before every step
+    (``FusedAdamW``; the reference does not clip, so None, the default, is its step)."""
+
     def __init__(self, dataloader, device, num_epochs, nz, generator, generator_name, discriminator,
-                 discriminator_name, rng=None):
+                 discriminator_name, rng=None, max_grad_norm=None):
         self.dataloader = dataloader
         self.device = torch.device(device)
         self.num_epochs = num_epochs
@@ -52,7 +55,11 @@ class Train(CheckpointMixin):
         self.generator, self.generator_name = generator, generator_name
         self.discriminator, self.discriminator_name = discriminator, discriminator_name
         self.rng = rng if rng is not None else DeviceRNG(self.device)
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0:
+            raise ValueError(f"max_grad_norm {max_grad_norm}")
         self.optimizer_G, self.optimizer_D = self.make_optimizers()
+        if max_grad_norm is not None:
+            self.optimizer_G.max_grad_norm = self.optimizer_D.max_grad_norm = max_grad_norm
         # epoch bookkeeping of train/trainunits.py:25-28 (checkpoint names and resume)
         self.epoch, self.i = 0, 0
         try:

@@ -267,6 +267,91 @@ int ganamd_adamw(float* p, const float* g, float* m, float* v, long n, int32_t* 
                  float beta2, float eps, float weight_decay, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Group norm with its activation (per-sample statistics: what a critic under the per-sample
+ * gradient penalty can use where BatchNorm cannot), twice differentiable.
+ *   xh = (x - mean) * rstd over the L * C/G values of a (sample, group), biased variance,
+ *   y = act(xh * w[c] + b[c])
+ * Maps: GANAMD_NORM_ROWS x[b][l][c] (channels last), GANAMD_NORM_PLANES x[c][b][l] (channel rows).
+ * x, y and the data gradients are in dtype; w, b, slope and their gradients in param_dtype
+ * (w NULL: ones, b NULL: zeros).  Statistics, sums and coefficients: 32 or 64 bits.
+ * stats: double [B][G][2] = mean, rstd, written by the forward, read by the other two.
+ * Every entry point takes any alignment of its data down to one element.
+ * ------------------------------------------------------------------------------------- */
+#define GANAMD_F32 0
+#define GANAMD_BF16 1
+#define GANAMD_F16 2
+
+#define GANAMD_NORM_ROWS 0
+#define GANAMD_NORM_PLANES 1
+
+#define GANAMD_NORM_NONE 0
+#define GANAMD_NORM_SILU 1
+#define GANAMD_NORM_LEAKY 2   /* z > 0 ? z : slope * z, one constant slope (0: ReLU) */
+#define GANAMD_NORM_PRELU 3   /* the same with slopes per channel, which have a gradient */
+
+typedef struct ganamd_norm_desc {
+  int64_t L;            /* positions per (sample, channel): H * W; at most 2^30 */
+  int32_t B, C, G;      /* G divides C */
+  int32_t layout, dtype, param_dtype, act;
+  float slope;          /* GANAMD_NORM_LEAKY */
+  float eps;            /* > 0 */
+} ganamd_norm_desc;
+
+/* Workspace bytes of the forward (op 0), backward (1) and double backward (2); may be 0. */
+int ganamd_group_norm_workspace(const ganamd_norm_desc* d, int op, size_t* bytes);
+/* The launch a call takes: info[10] = {one-launch form, vector width, threads, threads across /
+ * planes per block, positions in flight, channels per tile, tiles, chunks, positions per chunk,
+ * samples per slice} (introspection for tests). */
+int ganamd_group_norm_plan_info(const ganamd_norm_desc* d, int op, int* info);
+int ganamd_group_norm_fwd(const ganamd_norm_desc* d, const void* x, const void* w, const void* b, const void* slope,
+                          void* y, double* stats, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* Any output may be NULL (not wanted).  accumulate: gw, gb, gslope are added to (gx is written). */
+int ganamd_group_norm_bwd(const ganamd_norm_desc* d, const void* gy, const void* x, const void* w, const void* b,
+                          const void* slope, const double* stats, void* gx, void* gw, void* gb, void* gslope,
+                          int accumulate, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* The gradients of <ggx, gx> + <ggw, gw> + <ggb, gb> + <ggslope, gslope>, gx .. gslope the backward's
+ * outputs as functions of gy, x, w, b and slope: what the gradient penalty's second backward needs
+ * (wgangp.py:45-54,69).  ggw, ggb, ggslope may be NULL (zero); g_w, g_b, g_slope may be NULL. */
+int ganamd_group_norm_bwd_bwd(const ganamd_norm_desc* d, const void* ggx, const void* ggw, const void* ggb,
+                              const void* ggslope, const void* gy, const void* x, const void* w, const void* b,
+                              const void* slope, const double* stats, void* g_gy, void* g_x, void* g_w, void* g_b,
+                              void* g_slope, int accumulate, void* workspace, size_t workspace_bytes,
+                              hipStream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * The norm of many gradient tensors together and their clipping by it:
+ *   norm = sqrt(sum of all squares) (GANAMD_NORM_L2, summed in 64 bits) or the largest magnitude
+ *   (GANAMD_NORM_MAX; a NaN anywhere is the result), c = min(1, max_norm / (norm + 1e-6)),
+ *   out = c * p  (torch.nn.utils.clip_grad_norm_; with a norm of infinity c is 0, with NaN NaN)
+ * `list` is a HOST array, read during the call only.  Tensors of any count, n >= 0 elements each
+ * (densely stored), any alignment down to one element.  out may be p (in place) or a tensor of the
+ * same type or fp32; outputs must not share memory with each other or with other inputs
+ * (GANAMD_EINVAL).  norm: one float on the device.
+ * ------------------------------------------------------------------------------------- */
+#define GANAMD_NORM_L2 0
+#define GANAMD_NORM_MAX 1
+
+typedef struct ganamd_tensor {
+  const void* p;
+  void* out;          /* ganamd_grad_clip */
+  int64_t n;
+  int32_t dtype, out_dtype;   /* GANAMD_F32, _BF16, _F16 */
+} ganamd_tensor;
+
+size_t ganamd_grad_norm_workspace(const ganamd_tensor* list, int n);
+int ganamd_grad_norm(const ganamd_tensor* list, int n, int kind, float* norm, void* workspace, size_t workspace_bytes,
+                     hipStream_t stream);
+int ganamd_grad_clip(const ganamd_tensor* list, int n, int kind, float max_norm, float* norm, void* workspace,
+                     size_t workspace_bytes, hipStream_t stream);
+
+/* ganamd_adamw on c * g, c as above from the norm of the whole buffer g (which stays as it is);
+ * norm (one float on the device) receives it.  Two launches. */
+size_t ganamd_adamw_clip_workspace(void);
+int ganamd_adamw_clip(float* p, const float* g, float* m, float* v, long n, int32_t* step, double lr, double beta1,
+                      double beta2, double eps, double weight_decay, float max_norm, float* norm, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------------------
  * Grouped small GEMMs over a static tile list (the generator's style bank: the 519 per-conv
  * style MLPs and demodulation products of generator_13_5.py:223-227,239-242 in one launch).
  *   C[c_off + r*ldc + n] (=|+=) epi( sum_k A(r,k) * B(k,n) ),  r < rows, n < cols (each <= 64)
