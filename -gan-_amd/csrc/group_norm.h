@@ -233,68 +233,85 @@ struct Map {
 };
 
 // ------------------------------------------------------------------ per-channel constants
-__device__ __forceinline__ float kink(double mean, double rw, double b, bool& neg) {
+__device__ __forceinline__ float kink(double mean, double rw, double b, float& sg) {
   const float a = (float)rw;
-  neg = a < 0.f;
+  sg = a < 0.f ? -1.f : 1.f;
   if (a == 0.f) return b > 0.0 ? -INFINITY : NAN;      // z = b whatever x is
-  const double x0 = neg ? b / rw - mean : mean - b / rw;
+  const double x0 = a < 0.f ? b / rw - mean : mean - b / rw;
   const float t = (float)x0;
   return (double)t <= x0 ? nextafterf(t, INFINITY) : t;
 }
 
 // What the activation needs of a channel: d = x - mf; z = d * a + o (o carries the part of the
-// mean below fp32); the kink's threshold on x (on -x where a < 0), and its slope.
-template <int ACT>
+// mean below fp32); the kink's threshold tf on sg * x (sg: the sign of a), and its slope k.
+// A block's first threads make them, one channel each, and all read theirs from LDS (put / get:
+// field-major, `n` channels a field).
+template <int MODE, int ACT>
 struct Chan {
-  float mf, a, o, tf, k;
-  bool neg;
-  double xo;          // xh = r d + xo
+  static constexpr bool Z = MODE == FWD || ACT != KINK;       // uses z
+  static constexpr bool SIGN = MODE != FWD && ACT != SILU;    // uses the exact sign of z
+  static constexpr int N = 6;
+  float mf, a, o, tf, sg, k;
   __device__ __forceinline__ void set(const Args& g, double mean, double r, int c) {
     const float w = g.w ? loadp(g.w, g.pdt, c) : 1.f, bb = g.b ? loadp(g.b, g.pdt, c) : 0.f;
     mf = (float)mean;
     const double rw = r * (double)w;
-    xo = ((double)mf - mean) * r;
     a = (float)rw;
-    o = (float)((double)bb + xo * (double)w);
+    o = (float)((double)bb + ((double)mf - mean) * rw);
     k = 1.f;
     tf = 0.f;
-    neg = false;
-    if (ACT != SILU) {
-      k = g.slope ? loadp(g.slope, g.pdt, c) : g.cslope;
-      tf = kink(mean, rw, (double)bb, neg);
+    sg = 1.f;
+    if (ACT != SILU) k = g.slope ? loadp(g.slope, g.pdt, c) : g.cslope;
+    if (SIGN) tf = kink(mean, rw, (double)bb, sg);
+  }
+  template <class F>
+  __device__ __forceinline__ void fields(F f) {
+    f(0, mf);
+    f(1, a);
+    if (Z) f(2, o);
+    if (SIGN) {
+      f(3, tf);
+      f(4, sg);
     }
+    if (ACT != SILU) f(5, k);
+  }
+  __device__ __forceinline__ void put(float* t, int n, int c) {
+    fields([&](int i, float& v) { t[i * n + c] = v; });
+  }
+  __device__ __forceinline__ void get(const float* t, int n, int c) {
+    fields([&](int i, float& v) { v = t[i * n + c]; });
   }
 };
 
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
-template <int ACT>
-__device__ __forceinline__ float act_fwd(const Chan<ACT>& c, float x) {
+template <int MODE, int ACT>
+__device__ __forceinline__ float act_fwd(const Chan<MODE, ACT>& c, float x) {
   const float z = (x - c.mf) * c.a + c.o;
   if (ACT == SILU) return z * sigmoid(z);
   return z > 0.f ? z : c.k * z;
 }
 // g = gy a'(z); t = gy a''(z) (SILU) or gy [z <= 0] (kinked); z itself
-template <int ACT>
-__device__ __forceinline__ void act_bwd(const Chan<ACT>& c, float x, float d, float gy, float& g, float& t, float& z) {
+template <int MODE, int ACT>
+__device__ __forceinline__ void act_bwd(const Chan<MODE, ACT>& c, float x, float d, float gy, float& g, float& t, float& z) {
   z = d * c.a + c.o;
   if (ACT == SILU) {
     const float s = sigmoid(z), n = 1.f - s;
     g = gy * (s * (1.f + z * n));
     t = gy * (s * n * (2.f + z * (n - s)));
   } else {
-    const bool pos = (c.neg ? -x : x) >= c.tf;
+    const bool pos = c.sg * x >= c.tf;
     g = pos ? gy : c.k * gy;
     t = pos ? 0.f : gy;
   }
 }
-template <int ACT>
-__device__ __forceinline__ float act_d1(const Chan<ACT>& c, float x, float z) {
+template <int MODE, int ACT>
+__device__ __forceinline__ float act_d1(const Chan<MODE, ACT>& c, float x, float z) {
   if (ACT == SILU) {
     const float s = sigmoid(z);
     return s * (1.f + z * (1.f - s));
   }
-  return (c.neg ? -x : x) >= c.tf ? 1.f : c.k;
+  return c.sg * x >= c.tf ? 1.f : c.k;
 }
 
 // ------------------------------------------------------------------ sums over positions
@@ -312,7 +329,7 @@ template <>
 struct AccT<FWD> { typedef double type; };
 
 template <int MODE, int ACT, bool ROWS, class T, int V, int NC, int K, class A>
-__device__ __forceinline__ void accumulate(A (&acc)[K][NC], const Chan<ACT> (&ch)[NC], const Vec<T, V>& x,
+__device__ __forceinline__ void accumulate(A (&acc)[K][NC], const Chan<MODE, ACT> (&ch)[NC], const Vec<T, V>& x,
                                            const Vec<T, V>& gy, const Vec<T, V>& v) {
 #pragma unroll
   for (int j = 0; j < V; ++j) {
@@ -325,7 +342,7 @@ __device__ __forceinline__ void accumulate(A (&acc)[K][NC], const Chan<ACT> (&ch
     } else {
       const float d = xf - ch[c].mf;
       float g, t, z;
-      act_bwd<ACT>(ch[c], xf, d, gy.get(j), g, t, z);
+      act_bwd(ch[c], xf, d, gy.get(j), g, t, z);
       if constexpr (MODE == BWD) {
         acc[0][c] += g;
         acc[1][c] = fmaf(g, d, acc[1][c]);
@@ -490,15 +507,18 @@ __device__ __forceinline__ void dbl_coef(const Group& q, const double* m, const 
   co[4] = -2.0 * q.r * m[1] * m[3] + t[1] * invN + t[2] * invN;
 }
 
-// The elementwise pass's coefficients of one channel.
+// The elementwise pass's coefficients of one channel; the first moment of a slope's gradient needs
+// no z there, so a backward's SLOPE is its KINK.
 template <int MODE, int ACT>
 struct Lin {
-  Chan<ACT> ch;
+  typedef Chan<MODE, MODE == BWD && ACT == SLOPE ? KINK : ACT> C;
+  static constexpr int N = C::N + (MODE == FWD ? 0 : MODE == BWD ? 2 : 7);
+  C ch;
   float B1, C1;                     // BWD: gx = g a + d B1 + C1
   float H2, H3, G1, V1, D1, K1, cs; // DBL: h = v a + d H2 + H3; g_x = t a + g G1 + v V1 + d D1 + K1
   __device__ __forceinline__ void set(const Args& g, double mean, double r, const double* co, int c) {
     ch.set(g, mean, r, c);
-    const double w = param(g.w, g.pdt, c, 1.0), xo = ch.xo;
+    const double w = param(g.w, g.pdt, c, 1.0), xo = ((double)ch.mf - mean) * r;
     if (MODE == BWD) {
       B1 = (float)(-r * r * co[1]);
       C1 = (float)(-r * (co[0] + xo * co[1]));
@@ -514,6 +534,29 @@ struct Lin {
       cs = ACT == SLOPE ? (float)param(g.cs, g.pdt, c, 0.0) : 0.f;
     }
   }
+  template <class F>
+  __device__ __forceinline__ void fields(F f) {
+    constexpr int n = C::N;
+    ch.fields(f);
+    if (MODE == BWD) {
+      f(n, B1);
+      f(n + 1, C1);
+    } else if (MODE == DBL) {
+      f(n, H2);
+      f(n + 1, H3);
+      f(n + 2, G1);
+      f(n + 3, V1);
+      f(n + 4, D1);
+      f(n + 5, K1);
+      if (ACT == SLOPE) f(n + 6, cs);
+    }
+  }
+  __device__ __forceinline__ void put(float* t, int n, int c) {
+    fields([&](int i, float& v) { t[i * n + c] = v; });
+  }
+  __device__ __forceinline__ void get(const float* t, int n, int c) {
+    fields([&](int i, float& v) { v = t[i * n + c]; });
+  }
 };
 
 template <int MODE, int ACT, bool ROWS, class T, int V, int NC>
@@ -525,21 +568,21 @@ __device__ __forceinline__ void apply(const Lin<MODE, ACT> (&ln)[NC], const Vec<
     const Lin<MODE, ACT>& l = ln[ROWS ? j : 0];
     const float xf = x.get(j);
     if constexpr (MODE == FWD) {
-      f1[j] = act_fwd<ACT>(l.ch, xf);
+      f1[j] = act_fwd(l.ch, xf);
     } else {
       const float d = xf - l.ch.mf;
       float g, t, z;
-      act_bwd<ACT>(l.ch, xf, d, gy.get(j), g, t, z);
+      act_bwd(l.ch, xf, d, gy.get(j), g, t, z);
       if constexpr (MODE == BWD) {
         f1[j] = fmaf(g, l.ch.a, fmaf(d, l.B1, l.C1));
       } else {
         const float vf = v.get(j);
         const float h = fmaf(vf, l.ch.a, fmaf(d, l.H2, l.H3));
-        float gg = act_d1<ACT>(l.ch, xf, z) * h, tt = 0.f;
+        float gg = act_d1(l.ch, xf, z) * h, tt = 0.f;
         if (ACT == SILU) tt = t * h;
         if (ACT == SLOPE) {
           tt = l.cs * t;
-          if (!((l.ch.neg ? -xf : xf) >= l.ch.tf)) gg = fmaf(l.cs, z, gg);
+          if (!(l.ch.sg * xf >= l.ch.tf)) gg = fmaf(l.cs, z, gg);
         }
         f1[j] = gg;
         f2[j] = fmaf(tt, l.ch.a, fmaf(g, l.G1, fmaf(vf, l.V1, fmaf(d, l.D1, l.K1))));
@@ -550,15 +593,116 @@ __device__ __forceinline__ void apply(const Lin<MODE, ACT> (&ln)[NC], const Vec<
   if constexpr (MODE == DBL) o2.put(f2);
 }
 
-template <int MODE, int ACT, int NC>
-__device__ __forceinline__ void set_chan(const Args& a, Chan<ACT> (&ch)[NC], const double* stats_b, int c0) {
+// ------------------------------------------------------------------ shared by the kernels
+// A tile's channel constants for the sums (BWD, DBL): made in `tab`, read by every thread.
+template <int MODE, int ACT, bool ROWS, int V, int NC>
+__device__ __forceinline__ void load_chan(const Args& a, const Map<ROWS, V>& m, long b, int c0, float* tab,
+                                          Chan<MODE, ACT> (&ch)[NC]) {
   if constexpr (MODE != FWD) {
+    const int wid = min(a.CT, a.C - c0);
+    for (int c = threadIdx.x; c < wid; c += blockDim.x) {
+      const double* s = a.stats + 2 * (b * a.G + (c0 + c) / a.Cg);
+      Chan<MODE, ACT> q;
+      q.set(a, s[0], s[1], c0 + c);
+      q.put(tab, a.CT, c);
+    }
+    __syncthreads();
+    if (m.active) {
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const double* s = stats_b + 2 * ((c0 + j) / a.Cg);
-      ch[j].set(a, s[0], s[1], c0 + j);
+      for (int j = 0; j < NC; ++j) ch[j].get(tab, a.CT, max(m.slot + j, 0));   // (a moved-back front is not counted)
+    }
+    __syncthreads();                       // tab's memory becomes the sums'
+  }
+}
+
+// The same for the elementwise pass; co: the tile's first group's coefficients, 8 a group.
+template <int MODE, int ACT, bool ROWS, int V, int NC>
+__device__ __forceinline__ void load_lin(const Args& a, const Map<ROWS, V>& m, long b, int c0, const double* st,
+                                         int st_step, const double* co, float* tab, Lin<MODE, ACT> (&ln)[NC]) {
+  const int wid = min(a.CT, a.C - c0), g0 = c0 / a.Cg;
+  for (int c = threadIdx.x; c < wid; c += blockDim.x) {
+    const int g = (c0 + c) / a.Cg - g0;
+    Lin<MODE, ACT> q;
+    q.set(a, st[(long)g * st_step], st[(long)g * st_step + 1], co + 8L * g, c0 + c);
+    q.put(tab, a.CT, c);
+  }
+  __syncthreads();
+  if (m.active) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) ln[j].get(tab, a.CT, max(m.slot + j, 0));      // (nor stored)
+  }
+}
+
+// Groups c0 / Cg .. of sample b, a wave each, from their channels' sums chan[k * stride + c]:
+// statistics or coefficients to gco[8 a group], a sample's terms of the parameter gradients to par.
+template <int MODE, int ACT, class A>
+__device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int ng, const A* chan, long stride,
+                                              double* gco) {
+  const int lane = threadIdx.x & 63, nw = blockDim.x >> 6, g0 = c0 / a.Cg;
+  const double invN = 1.0 / ((double)a.L * a.Cg);
+  for (int gi = threadIdx.x >> 6; gi < ng; gi += nw) {
+    const int cg = gi * a.Cg;
+    double* st = a.stats + 2 * (b * a.G + g0 + gi);
+    double* co = gco + 8L * gi;
+    if constexpr (MODE == FWD) {
+      double s = 0, q = 0;
+      for (int c = lane; c < a.Cg; c += 64) {
+        s += chan[cg + c];
+        q += chan[stride + cg + c];
+      }
+      s = wave_sum(s);
+      q = wave_sum(q);
+      const double mean = s * invN, var = fmax(q * invN - mean * mean, 0.0);
+      const double nan = s - s + (q - q);            // fmax drops a NaN: put it back
+      const double r = 1.0 / sqrt(var + nan + (double)a.eps);
+      if (lane == 0) {
+        co[0] = mean;
+        co[1] = r;
+        st[0] = mean;
+        st[1] = r;
+      }
+    } else {
+      const Group q = group_of(st[0], st[1]);
+      const int cc = c0 + cg;
+      double m1[4] = {0, 0, 0, 0};
+      for (int c = lane; c < a.Cg; c += 64) {
+        double terms[3];
+        sweep1<MODE, ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * stride + cg + c]; }, m1, terms);
+        if (MODE == BWD && a.par)
+#pragma unroll
+          for (int k = 0; k < Sums<BWD, ACT>::K; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
+      }
+#pragma unroll
+      for (int k = 0; k < (MODE == BWD ? 2 : 4); ++k) m1[k] = wave_sum(m1[k]) * invN;
+      if (MODE == BWD) {
+        if (lane == 0) {
+          co[0] = m1[0];
+          co[1] = m1[1];
+        }
+      } else {
+        double m2[3] = {0, 0, 0};
+        for (int c = lane; c < a.Cg; c += 64) {
+          double terms[3];
+          sweep2<ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * stride + cg + c]; }, m1, m2, terms);
+          if (a.par)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) m2[k] = wave_sum(m2[k]);
+        if (lane == 0) dbl_coef(q, m1, m2, invN, co);
+      }
     }
   }
+}
+
+template <int MODE, int ACT, bool ROWS, class T, int V, int NC>
+__device__ __forceinline__ void write(const Args& a, const Lin<MODE, ACT> (&ln)[NC], long at, int skip,
+                                      const Vec<T, V>& x, const Vec<T, V>& gy, const Vec<T, V>& v) {
+  Vec<T, V> o1, o2;
+  apply<MODE, ACT, ROWS, T, V, NC>(ln, x, gy, v, o1, o2);
+  if (MODE != BWD || a.o1) store(static_cast<T*>(a.o1) + at, o1, skip);
+  if constexpr (MODE == DBL) store(static_cast<T*>(a.o2) + at, o2, skip);
 }
 
 // ------------------------------------------------------------------ the resident form
@@ -573,8 +717,9 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
   const Map<ROWS, V> m(a, b, tile);
   const int gt = a.CT / a.Cg;                       // groups of a tile (the last may hold fewer)
   double* gco = reinterpret_cast<double*>(lds);     // [gt][8] (FWD: mean, r)
-  A* chan = reinterpret_cast<A*>(gco + gt * 8);     // [K][CT]
-  A* sh = chan + K * a.CT + (K * a.CT & 1);
+  float* tab = reinterpret_cast<float*>(gco + gt * 8);
+  A* chan = reinterpret_cast<A*>(tab);              // [K][CT]
+  A* sh = chan + K * a.CT;
   const T* px = static_cast<const T*>(a.x);
   const T* pg = static_cast<const T*>(a.gy);
   const T* pv = static_cast<const T*>(a.v);
@@ -583,23 +728,20 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
 #pragma unroll
   for (int k = 0; k < RMAX; ++k) {
     const int i = m.p + k * a.P;
+    int skip = V;
     if (m.active && i < m.npos) {
-      int skip;
       const long at = m.at(i, skip);
       x[k] = load<T, V>(px + at);
       if constexpr (MODE >= BWD) gy[k] = load<T, V>(pg + at);
       if constexpr (MODE == DBL) v[k] = load<T, V>(pv + at);
-      if (MODE == FWD) x[k].zero_front(skip);
-      if constexpr (MODE >= BWD) gy[k].zero_front(skip);
-      if constexpr (MODE == DBL) v[k].zero_front(skip);
-    } else {
-      x[k].zero_front(V);
-      if constexpr (MODE >= BWD) gy[k].zero_front(V);
-      if constexpr (MODE == DBL) v[k].zero_front(V);
     }
+    if (MODE == FWD || skip == V) x[k].zero_front(skip);
+    if constexpr (MODE >= BWD) gy[k].zero_front(skip);
+    if constexpr (MODE == DBL) v[k].zero_front(skip);
   }
-  Chan<ACT> ch[NC];
-  set_chan<MODE>(a, ch, a.stats + 2 * b * a.G, m.ch);
+  const int c0 = tile * a.CT, g0 = c0 / a.Cg, ng = min(gt, a.G - g0);
+  Chan<MODE, ACT> ch[NC];
+  load_chan<MODE, ACT, ROWS, V, NC>(a, m, b, c0, tab, ch);
   A acc[K][NC];
 #pragma unroll
   for (int k = 0; k < K; ++k)
@@ -607,7 +749,7 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
     for (int j = 0; j < NC; ++j) acc[k][j] = 0;
 #pragma unroll
   for (int k = 0; k < RMAX; ++k)
-    if (k == 0 || k * a.P < m.npos)
+    if (m.active && (k == 0 || k * a.P < m.npos))
       accumulate<MODE, ACT, ROWS, T, V, NC>(acc, ch, x[k], gy[MODE >= BWD ? k : 0], v[MODE == DBL ? k : 0]);
 #pragma unroll
   for (int k = 0; k < RMAX; ++k) {
@@ -616,82 +758,21 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
     if constexpr (MODE == DBL) v[k].pin();
   }
   fold<ROWS, V, K, NC>(a, m, acc, sh, chan);
-
-  // groups: one wave each
-  const int lane = threadIdx.x & 63, nw = blockDim.x >> 6;
-  const int c0 = tile * a.CT, g0 = c0 / a.Cg, ng = min(gt, a.G - g0);
-  const double invN = 1.0 / ((double)a.L * a.Cg);
-  for (int gi = threadIdx.x >> 6; gi < ng; gi += nw) {
-    const int cg = gi * a.Cg;
-    double* st = a.stats + 2 * (b * a.G + g0 + gi);
-    if constexpr (MODE == FWD) {
-      double s = 0, q = 0;
-      for (int c = lane; c < a.Cg; c += 64) {
-        s += chan[cg + c];
-        q += chan[a.CT + cg + c];
-      }
-      s = wave_sum(s);
-      q = wave_sum(q);
-      const double mean = s * invN, var = fmax(q * invN - mean * mean, 0.0);
-      const double nan = s - s + (q - q);            // fmax drops a NaN: put it back
-      const double r = 1.0 / sqrt(var + nan + (double)a.eps);
-      if (lane == 0) {
-        gco[gi * 8] = mean;
-        gco[gi * 8 + 1] = r;
-        st[0] = mean;
-        st[1] = r;
-      }
-    } else {
-      const Group q = group_of(st[0], st[1]);
-      const int cc = c0 + cg;
-      double m1[4] = {0, 0, 0, 0};
-      for (int c = lane; c < a.Cg; c += 64) {
-        double terms[3];
-        sweep1<MODE, ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * a.CT + cg + c]; }, m1, terms);
-        if (MODE == BWD && a.par)
-          for (int k = 0; k < Sums<BWD, ACT>::K; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
-      }
-      for (int k = 0; k < (MODE == BWD ? 2 : 4); ++k) m1[k] = wave_sum(m1[k]) * invN;
-      if (MODE == BWD) {
-        if (lane == 0) {
-          gco[gi * 8] = m1[0];
-          gco[gi * 8 + 1] = m1[1];
-        }
-      } else {
-        double m2[3] = {0, 0, 0};
-        for (int c = lane; c < a.Cg; c += 64) {
-          double terms[3];
-          sweep2<ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * a.CT + cg + c]; }, m1, m2, terms);
-          if (a.par)
-            for (int k = 0; k < 3; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
-        }
-        for (int k = 0; k < 3; ++k) m2[k] = wave_sum(m2[k]);
-        if (lane == 0) dbl_coef(q, m1, m2, invN, gco + gi * 8);
-      }
-    }
-  }
+  finish_groups<MODE, ACT>(a, b, c0, ng, chan, (long)a.CT, gco);
   __syncthreads();
-  if (!m.active) return;
   Lin<MODE, ACT> ln[NC];
-#pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    const int c = m.ch + j, gi = c / a.Cg - g0;
-    if (gi >= 0 && gi < ng) {                        // (a moved-back vector's front lies in another tile)
-      const double* st = MODE == FWD ? gco + gi * 8 : a.stats + 2 * (b * a.G + g0 + gi);
-      ln[j].set(a, st[0], st[1], gco + gi * 8, c);
-    }
-  }
+  if (MODE == FWD)
+    load_lin<MODE, ACT, ROWS, V, NC>(a, m, b, c0, gco, 8, gco, tab, ln);
+  else
+    load_lin<MODE, ACT, ROWS, V, NC>(a, m, b, c0, a.stats + 2 * (b * a.G + g0), 2, gco, tab, ln);
+  if (!m.active) return;
 #pragma unroll
   for (int k = 0; k < RMAX; ++k) {
     const int i = m.p + k * a.P;
     if (i < m.npos) {
       int skip;
       const long at = m.at(i, skip);
-      Vec<T, V> o1, o2;
-      apply<MODE, ACT, ROWS, T, V, NC>(ln, x[k], gy[MODE >= BWD ? k : 0], v[MODE == DBL ? k : 0], o1, o2);
-      if (MODE != BWD || a.o1) store(static_cast<T*>(a.o1) + at, o1, skip);
-      if constexpr (MODE == DBL)
-        if (a.o2) store(static_cast<T*>(a.o2) + at, o2, skip);
+      write<MODE, ACT, ROWS, T, V, NC>(a, ln, at, skip, x[k], gy[MODE >= BWD ? k : 0], v[MODE == DBL ? k : 0]);
     }
   }
 }
@@ -699,183 +780,153 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
 // ------------------------------------------------------------------ the split form
 constexpr int kNT = 512;
 
+// The loop of both passes over a chunk: U positions at a time, the next ones loaded before the
+// present ones are used; `first` runs between the first loads and their use.
+template <int MODE, bool ROWS, class T, int V, int U, class First, class Use>
+__device__ __forceinline__ void stream(const Args& a, const Map<ROWS, V>& m, int lo, int hi, First first, Use use) {
+  const T* px = static_cast<const T*>(a.x);
+  const T* pg = static_cast<const T*>(a.gy);
+  const T* pv = static_cast<const T*>(a.v);
+  Vec<T, V> x[U], gy[MODE >= BWD ? U : 1], v[MODE == DBL ? U : 1];
+  long at[U];
+  int skip[U];
+  const int step = U * a.P;
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * a.P;
+      skip[u] = V;
+      if (i < hi) {
+        at[u] = m.at(i, skip[u]);
+        x[u] = load<T, V>(px + at[u]);
+        if constexpr (MODE >= BWD) gy[u] = load<T, V>(pg + at[u]);
+        if constexpr (MODE == DBL) v[u] = load<T, V>(pv + at[u]);
+      }
+    }
+  };
+  if (m.active) fetch(lo + m.p);
+  first();
+  if (!m.active) return;
+  for (int i0 = lo + m.p; i0 < hi; i0 += step) {
+    Vec<T, V> cx[U], cg[MODE >= BWD ? U : 1], cv[MODE == DBL ? U : 1];
+    long ca[U];
+    int cs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      cx[u] = x[u];
+      if constexpr (MODE >= BWD) cg[u] = gy[u];
+      if constexpr (MODE == DBL) cv[u] = v[u];
+      ca[u] = at[u];
+      cs[u] = skip[u];
+    }
+    if (i0 + step < hi) fetch(i0 + step);
+#pragma unroll
+    for (int u = 0; u < U; ++u) use(ca[u], cs[u], cx[u], cg[MODE >= BWD ? u : 0], cv[MODE == DBL ? u : 0]);
+  }
+}
+
 // blockIdx.x = (sample, tile, chunk), chunk fastest
 template <int MODE, int ACT, bool ROWS, class T, int V>
 __global__ __launch_bounds__(kNT) void sums_kernel(Args a) {
   typedef typename AccT<MODE>::type A;
-  constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K, U = 4;
+  constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K, U = MODE == DBL ? 2 : 4;
   extern __shared__ __align__(16) char lds[];
   const int s = blockIdx.x % a.S, tile = blockIdx.x / a.S % a.nct;
   const int bi = blockIdx.x / a.S / a.nct;
   const long b = a.b0 + bi;
   const Map<ROWS, V> m(a, b, tile);
+  float* tab = reinterpret_cast<float*>(lds);
   A* chan = reinterpret_cast<A*>(lds);
-  A* sh = chan + K * a.CT + (K * a.CT & 1);
-  const T* px = static_cast<const T*>(a.x);
-  const T* pg = static_cast<const T*>(a.gy);
-  const T* pv = static_cast<const T*>(a.v);
-  Chan<ACT> ch[NC];
-  set_chan<MODE>(a, ch, a.stats + 2 * b * a.G, m.ch);
+  A* sh = chan + K * a.CT;
+  const int c0 = tile * a.CT, wid = min(a.CT, a.C - c0);
+  const int hi = (int)min((long)m.npos, (long)(s + 1) * a.per);
+  Chan<MODE, ACT> ch[NC];
   A acc[K][NC];
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int j = 0; j < NC; ++j) acc[k][j] = 0;
-  const int hi = (int)min((long)m.npos, (long)(s + 1) * a.per);
-  if (m.active) {
-    for (int i0 = s * a.per + m.p; i0 < hi; i0 += U * a.P) {
-      Vec<T, V> x[U], gy[MODE >= BWD ? U : 1], v[MODE == DBL ? U : 1];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * a.P;
-        int skip = V;
-        if (i < hi) {
-          const long at = m.at(i, skip);
-          x[u] = load<T, V>(px + at);
-          if constexpr (MODE >= BWD) gy[u] = load<T, V>(pg + at);
-          if constexpr (MODE == DBL) v[u] = load<T, V>(pv + at);
-        }
-        if (MODE == FWD || skip == V) x[u].zero_front(skip);
-        if constexpr (MODE >= BWD) gy[u].zero_front(skip);
-        if constexpr (MODE == DBL) v[u].zero_front(skip);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        accumulate<MODE, ACT, ROWS, T, V, NC>(acc, ch, x[u], gy[MODE >= BWD ? u : 0], v[MODE == DBL ? u : 0]);
-    }
-  }
+  stream<MODE, ROWS, T, V, U>(
+      a, m, s * a.per, hi, [&] { load_chan<MODE, ACT, ROWS, V, NC>(a, m, b, c0, tab, ch); },
+      [&](long, int skip, Vec<T, V>& x, Vec<T, V>& gy, Vec<T, V>& v) {
+        if (MODE == FWD || skip == V) x.zero_front(skip);
+        if constexpr (MODE >= BWD) gy.zero_front(skip);
+        if constexpr (MODE == DBL) v.zero_front(skip);
+        accumulate<MODE, ACT, ROWS, T, V, NC>(acc, ch, x, gy, v);
+      });
   fold<ROWS, V, K, NC>(a, m, acc, sh, chan);
-  const int c0 = tile * a.CT, wid = min(a.CT, a.C - c0);
   A* part = reinterpret_cast<A*>(a.part) + ((long)bi * a.S + s) * K * a.C;
   for (int i = threadIdx.x; i < K * wid; i += blockDim.x)
     part[(long)(i / wid) * a.C + c0 + i % wid] = chan[i / wid * a.CT + i % wid];
 }
 
-// Block (sample, group): the chunks' sums folded, in double and in one order; the group's coefficients.
+// Many chunks: every 32 of a channel's into the first of them, so that the group blocks' loop is short.
+constexpr int kFold = 32;
+
+template <class A>
+__global__ __launch_bounds__(256) void chunk_kernel(A* part, int S, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x, s0 = blockIdx.y * kFold;
+  if (i >= n) return;
+  A* p = part + ((long)blockIdx.z * S + s0) * n + i;
+  double t = 0;
+#pragma unroll 8
+  for (int s = 0; s < min(kFold, S - s0); ++s) t += (double)p[(long)s * n];
+  *p = (A)t;
+}
+
+// Block (sample, gpb groups): the chunks' sums folded in double and in one order into the first
+// chunk's place, then the groups' statistics or coefficients.
 template <int MODE, int ACT>
-__global__ __launch_bounds__(256) void group_kernel(Args a) {
+__global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) {
   typedef typename AccT<MODE>::type A;
   constexpr int K = Sums<MODE, ACT>::K;
-  __shared__ double red[4][4], sh[256];
-  extern __shared__ __align__(16) char lds[];
-  double* chan = reinterpret_cast<double*>(lds);      // [K][min(Cg, 256)]: a pass of channels
-  const int gi = blockIdx.x % a.G, bi = blockIdx.x / a.G;
+  const int nb = (a.G + gpb - 1) / gpb, g0 = blockIdx.x % nb * gpb, bi = blockIdx.x / nb;
   const long b = a.b0 + bi;
-  const int tid = threadIdx.x;
-  int cw = 1;
-  while (cw < a.Cg && cw < 256) cw *= 2;
-  const int sw = 256 / cw, ci = tid % cw, si = tid / cw;
-  const A* part = reinterpret_cast<const A*>(a.part) + (long)bi * a.S * K * a.C + gi * a.Cg;
-  double* st = a.stats + 2 * (b * a.G + gi);
-  Group q = {0, 0, 0, 0};
-  if (MODE != FWD) q = group_of(st[0], st[1]);
-  const double invN = 1.0 / ((double)a.L * a.Cg);
-  double m1[4] = {0, 0, 0, 0}, m2[3] = {0, 0, 0};
-  for (int sweep = 0; sweep < (MODE == DBL ? 2 : 1); ++sweep) {
-    for (int cb = 0; cb < a.Cg; cb += cw) {
-      const int c = cb + ci;
-      if (sweep == 0 || a.Cg > cw) {
-        for (int k = 0; k < K; ++k) {
-          double t = 0;
-          if (c < a.Cg)
-            for (int s = si; s < a.S; s += sw) t += (double)part[((long)s * K + k) * a.C + c];
-          __syncthreads();
-          sh[tid] = t;
-          __syncthreads();
-          if (si == 0) {
-            for (int i = 1; i < sw; ++i) t += sh[i * cw + ci];
-            chan[k * cw + ci] = t;
-          }
-        }
+  const int ng = min(gpb, a.G - g0), nc = ng * a.Cg, pairs = K * nc, ns = (a.S + sstep - 1) / sstep;
+  A* part = reinterpret_cast<A*>(a.part) + (long)bi * a.S * K * a.C + g0 * a.Cg;
+  if (ns > 1) {
+    int sw = 1;                                       // lanes that share a channel's chunks
+    while (sw * 2 * pairs <= 256 && sw * 2 <= ns && sw < 64) sw *= 2;
+    const int q = threadIdx.x & (sw - 1);
+    const long hop = (long)sstep * K * a.C;
+    for (int i0 = 0; i0 < pairs; i0 += 256 / sw) {
+      const int i = i0 + threadIdx.x / sw;
+      A* p = part + (long)(i / nc) * a.C + i % nc;
+      double t = 0;
+      if (i < pairs) {
+#pragma unroll 8
+        for (int s = q; s < ns; s += sw) t += (double)p[s * hop];
       }
-      if (si == 0 && c < a.Cg) {                      // (reads back what this thread wrote)
-        const int cc = gi * a.Cg + c;
-        auto get = [&](int k) { return chan[k * cw + ci]; };
-        double terms[3] = {0, 0, 0};
-        if constexpr (MODE == FWD) {
-          m1[0] += get(0);
-          m1[1] += get(1);
-        } else if (sweep == 0) {
-          sweep1<MODE, ACT>(a, q, cc, get, m1, terms);
-        } else {
-          sweep2<ACT>(a, q, cc, get, m1, m2, terms);
-        }
-        if (MODE != FWD && a.par && (MODE == BWD || sweep == 1))
-          for (int k = 0; k < (MODE == BWD ? Sums<BWD, ACT>::K : 3); ++k)
-            a.par[(k * a.B + b) * a.C + cc] = (float)terms[k];
-      }
-    }
-    double* mm = sweep == 0 ? m1 : m2;
-    const int n = sweep == 0 ? 4 : 3;
-    for (int k = 0; k < n; ++k) {
-      const double t = wave_sum(mm[k]);
-      if ((tid & 63) == 0) red[k][tid >> 6] = t;
+      for (int o = sw / 2; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+      if (q == 0 && i < pairs) *p = (A)t;
     }
     __syncthreads();
-    for (int k = 0; k < n; ++k) mm[k] = (red[k][0] + red[k][1]) + (red[k][2] + red[k][3]);
-    __syncthreads();
-    if (MODE != FWD && sweep == 0)
-      for (int k = 0; k < 4; ++k) m1[k] *= invN;
   }
-  if (tid != 0) return;
-  double* co = a.coef + 8 * (b * a.G + gi);
-  if constexpr (MODE == FWD) {
-    const double mean = m1[0] * invN, var = fmax(m1[1] * invN - mean * mean, 0.0);
-    const double nan = m1[0] - m1[0] + (m1[1] - m1[1]);
-    st[0] = mean;
-    st[1] = 1.0 / sqrt(var + nan + (double)a.eps);
-  } else if constexpr (MODE == BWD) {
-    co[0] = m1[0];
-    co[1] = m1[1];
-  } else {
-    dbl_coef(q, m1, m2, invN, co);
-  }
+  // (FWD writes the statistics; the coefficients have their own place)
+  extern __shared__ __align__(16) double gco[];
+  finish_groups<MODE, ACT>(a, b, g0 * a.Cg, ng, part, (long)a.C, MODE == FWD ? gco : a.coef + 8 * (b * a.G + g0));
 }
 
 template <int MODE, int ACT, bool ROWS, class T, int V>
 __global__ __launch_bounds__(kNT) void apply_kernel(Args a) {
   constexpr int NC = ROWS ? V : 1, U = 2;
+  extern __shared__ __align__(16) char lds[];
   const int s = blockIdx.x % a.S, tile = blockIdx.x / a.S % a.nct;
   const long b = a.b0 + blockIdx.x / a.S / a.nct;
   const Map<ROWS, V> m(a, b, tile);
-  if (!m.active) return;
-  const T* px = static_cast<const T*>(a.x);
-  const T* pg = static_cast<const T*>(a.gy);
-  const T* pv = static_cast<const T*>(a.v);
-  Lin<MODE, ACT> ln[NC];
-#pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    const long g = b * a.G + (m.ch + j) / a.Cg;
-    ln[j].set(a, a.stats[2 * g], a.stats[2 * g + 1], a.coef + 8 * g, m.ch + j);
-  }
+  const int c0 = tile * a.CT;
   const int hi = (int)min((long)m.npos, (long)(s + 1) * a.per);
-  for (int i0 = s * a.per + m.p; i0 < hi; i0 += U * a.P) {
-    Vec<T, V> x[U], gy[MODE >= BWD ? U : 1], v[MODE == DBL ? U : 1];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * a.P;
-      if (i < hi) {
-        int skip;
-        const long at = m.at(i, skip);
-        x[u] = load<T, V>(px + at);
-        if constexpr (MODE >= BWD) gy[u] = load<T, V>(pg + at);
-        if constexpr (MODE == DBL) v[u] = load<T, V>(pv + at);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * a.P;
-      if (i < hi) {
-        int skip;
-        const long at = m.at(i, skip);
-        Vec<T, V> o1, o2;
-        apply<MODE, ACT, ROWS, T, V, NC>(ln, x[u], gy[MODE >= BWD ? u : 0], v[MODE == DBL ? u : 0], o1, o2);
-        if (MODE != BWD || a.o1) store(static_cast<T*>(a.o1) + at, o1, skip);
-        if constexpr (MODE == DBL)
-          if (a.o2) store(static_cast<T*>(a.o2) + at, o2, skip);
-      }
-    }
-  }
+  const long g0 = b * a.G + c0 / a.Cg;
+  Lin<MODE, ACT> ln[NC];
+  stream<MODE, ROWS, T, V, U>(
+      a, m, s * a.per, hi,
+      [&] {
+        load_lin<MODE, ACT, ROWS, V, NC>(a, m, b, c0, a.stats + 2 * g0, 2, a.coef + 8 * g0,
+                                         reinterpret_cast<float*>(lds), ln);
+      },
+      [&](long at, int skip, Vec<T, V>& x, Vec<T, V>& gy, Vec<T, V>& v) {
+        if (skip < V) write<MODE, ACT, ROWS, T, V, NC>(a, ln, at, skip, x, gy, v);
+      });
 }
 
 // ------------------------------------------------------------------ launches
@@ -889,7 +940,8 @@ struct Plan {
   int mode, act;
   bool rows, resident;
   int V, rmax, nt;
-  size_t lds, group_lds;
+  size_t lds, apply_lds;
+  int gpb, sstep;         // groups a folding block takes; chunks are folded by 32 before (or 1)
   int slice;              // samples per slice
 };
 
@@ -911,8 +963,16 @@ int launch_v(const Plan& p, const Args& a, long nb, hipStream_t st) {
   }
   const dim3 grid((unsigned)(nb * a.nct * a.S));
   hipLaunchKernelGGL((sums_kernel<MODE, ACT, ROWS, T, V>), grid, dim3(p.nt), p.lds, st, a);
-  hipLaunchKernelGGL((group_kernel<MODE, ACT>), dim3((unsigned)(nb * a.G)), dim3(256), p.group_lds, st, a);
-  if (MODE != BWD || a.o1) hipLaunchKernelGGL((apply_kernel<MODE, ACT, ROWS, T, V>), grid, dim3(p.nt), 0, st, a);
+  if (p.sstep > 1) {
+    typedef typename AccT<MODE>::type A;
+    const int n = Sums<MODE, ACT>::K * a.C;
+    hipLaunchKernelGGL(chunk_kernel<A>, dim3((n + 255) / 256, (a.S + kFold - 1) / kFold, (unsigned)nb), dim3(256), 0,
+                       st, reinterpret_cast<A*>(a.part), a.S, n);
+  }
+  hipLaunchKernelGGL((group_kernel<MODE, ACT>), dim3((unsigned)(nb * ((a.G + p.gpb - 1) / p.gpb))), dim3(256),
+                     MODE == FWD ? 64 * (size_t)p.gpb : 0, st, a, p.gpb, p.sstep);
+  if (MODE != BWD || a.o1)
+    hipLaunchKernelGGL((apply_kernel<MODE, ACT, ROWS, T, V>), grid, dim3(p.nt), p.apply_lds, st, a);
   return hipGetLastError() == hipSuccess ? GANAMD_OK : GANAMD_ELAUNCH;
 }
 

@@ -50,6 +50,7 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   const int K = mode == gn::FWD ? 2 : mode == gn::BWD ? (p.act == gn::SLOPE ? 3 : 2)
               : (p.act == gn::SILU ? 10 : p.act == gn::SLOPE ? 8 : 5);
   const size_t asz = mode == gn::FWD ? 8 : 4;
+  const int tabs = mode == gn::FWD ? 6 : mode == gn::BWD ? 8 : 13;      // fields of a channel's coefficients
   const int rcap = gn::resident_vectors(mode), most = gn::resident_threads(mode, p.rows);
   a.L = L; a.B = B; a.C = C; a.G = G; a.Cg = Cg; a.eps = d->eps; a.pdt = d->param_dtype;
   a.cslope = d->act == GANAMD_NORM_LEAKY ? d->slope : 1.f;
@@ -86,15 +87,15 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     a.S = 1;
     a.per = 0;
     const size_t sh = p.rows ? (size_t)a.P * a.CT : (size_t)K * 16;
-    p.lds = (size_t)(a.CT / Cg) * 64 + asz * ((size_t)K * a.CT + 1 + sh);
+    p.lds = (size_t)(a.CT / Cg) * 64 + std::max(asz * ((size_t)K * a.CT + sh), 4 * (size_t)tabs * a.CT);
     if (p.lds > 64 * 1024) p.resident = false;
   }
   if (!p.resident) {
     long npos;
     if (p.rows) {
       const long all = up_to(C, p.V);
-      // (a tile's channels: their sums, K each, and the fold's scratch share 64 KB)
-      a.nct = (int)std::max(up_to(all, gn::kNT), up_to(all * p.V * K * (long)asz, 24 * 1024));
+      // (a tile's channels: their sums or coefficients, and the fold's scratch, share 64 KB)
+      a.nct = (int)std::max(up_to(all, gn::kNT), up_to(all * p.V * std::max<long>(K * asz, 4 * tabs), 24 * 1024));
       a.TX = (int)up_to(all, a.nct);
       a.CT = a.TX * p.V;
       a.nct = (int)up_to(C, a.CT);
@@ -115,9 +116,11 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     a.per = (int)(up_to(up_to(npos, S), a.P) * a.P);
     a.S = (int)up_to(npos, a.per);
     const size_t sh = p.rows ? (size_t)a.P * a.CT : (size_t)K * 16;
-    p.lds = asz * ((size_t)K * a.CT + 1 + sh);
+    p.lds = std::max(asz * ((size_t)K * a.CT + sh), 4 * (size_t)tabs * a.CT);
+    p.apply_lds = 4 * (size_t)tabs * a.CT;
   }
-  p.group_lds = 8 * (size_t)K * std::min<long>(256, pow2_at_least(Cg));
+  p.gpb = (int)std::max<long>(1, std::min<long>(G, 256 / ((long)K * Cg)));
+  p.sstep = a.S > 2 * gn::kFold ? gn::kFold : 1;
   if (B * a.nct * a.S >= (1L << 31) || B * G >= (1L << 31) || p.lds > 64 * 1024) return false;
   // workspace
   size_t at = 0;

@@ -1615,10 +1615,21 @@ def _norm_backward(cfg, gy, x, w, b, slope, stats, gx, gw, gb, gs, accumulate):
                                         *wsarg(cfg.workspace(1, x.device)), stream()), "group_norm_bwd")
 
 
+def _in_flat(p) -> bool:
+    return p is not None and getattr(p if p._base is None else p._base, "_gan_flat", None) is not None
+
+
+def _norm_wants(args, need):
+    """Which parameter gradients a norm's backward makes.  One of a flat-buffer parameter is added to
+    that buffer, so it is only made where the engine asks for it (``wanted``; elsewhere a gradient
+    nobody asked for is dropped by the engine, which costs less than asking)."""
+    return [n and (not _in_flat(a) or wanted(a)) for n, a in zip(need, args)]
+
+
 def _param_targets(args, pars, need):
     """Where the gradients of a norm's parameters go: (buffers, accumulate) -- the flat gradient
     buffers when all wanted ones live there, new tensors otherwise (None: not wanted)."""
-    need = [n and wanted(a) for n, a in zip(need, args)]
+    need = _norm_wants(args, need)
     flat = [flat_grad(a) if n else None for n, a in zip(need, args)]
     if any(need) and all(f is not None for n, f in zip(need, flat) if n) and all(
             f.dtype == torch.float32 == p.dtype for f, p in zip(flat, pars) if f is not None):
@@ -1642,7 +1653,7 @@ class GroupNormAct(Function):
         x, w, b, slope, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         if torch.is_grad_enabled():                       # create_graph: differentiable once more
-            want = [n and wanted(a) for n, a in zip(need[1:4], ctx.args)]
+            want = _norm_wants(ctx.args, need[1:4])
             return (*GroupNormActBackward.apply(gy, x, *ctx.args, stats, ctx.cfg, want), None)
         gy = _c(gy)
         gx = torch.empty_like(x) if need[0] else None
