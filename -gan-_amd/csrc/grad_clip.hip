@@ -21,7 +21,7 @@
 namespace {
 
 constexpr int kNT = 256;
-constexpr long kChunkMin = 4096, kChunkMax = 65536;
+constexpr long kChunkMin = 4096, kChunkMax = 16384;
 constexpr int kFoldMax = 1024;      // partials that every scaling block folds by itself
 constexpr int kTable = 160;         // tensors of a launch (the arguments stay under 4 KB)
 constexpr int kStepBlocks = 1024;   // partials of the flat buffer's norm

@@ -1732,56 +1732,14 @@ def group_norm_act(x, groups: int, weight=None, bias=None, act: str = "none", sl
 _NORM_KINDS = {2.0: _lib.NORM_L2, float("inf"): _lib.NORM_MAX}
 
 
-def _dense(t) -> bool:
-    """Does ``t`` fill one block of memory, each element once, in whatever order of its dimensions?"""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if st != want:
-            return False
-        want *= n
-    return True
-
-
 def _tensor_list(what, tensors, out=None):
-    """The host table of a list of gradients (ganamd_tensor), checked."""
+    """The host table of a list of gradients (ganamd_tensor rows), checked (csrc/host.cpp)."""
     ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-
-    def bad(msg):
-        raise _lib.GanAmdError(f"{what}: {msg}")
-
-    def column(ts, name):
-        if not all(isinstance(t, torch.Tensor) for t in ts):
-            bad(f"{name} are tensors; got {[type(t).__name__ for t in ts if not isinstance(t, torch.Tensor)][0]}")
-        if not all(t.is_cuda for t in ts) or len(set(map(torch.Tensor.get_device, ts))) > 1:
-            bad(f"{name} are on one GPU; got {sorted({str(t.device) for t in ts})}")
-        try:
-            dt = [_DTYPES[t.dtype] for t in ts]
-        except KeyError as e:
-            bad(f"{name} are float32, bfloat16 or float16; got {e.args[0]}")
-        if not all(map(torch.Tensor.is_contiguous, ts)) and not all(map(_dense, ts)):
-            bad(f"{name} are stored densely; got strides {[t.stride() for t in ts if not _dense(t)][0]}")
-        return list(map(torch.Tensor.data_ptr, ts)), list(map(torch.Tensor.numel, ts)), dt
-
-    ptrs, ns, dts = column(ts, "gradients")
-    if out is None:
-        outs, odts, dst = ptrs, dts, ts
-    else:
-        dst = [out] if isinstance(out, torch.Tensor) else list(out)
-        if len(dst) != len(ts):
-            bad(f"{len(ts)} gradients, {len(dst)} outputs")
-        outs, ons, odts = column(dst, "outputs")
-        if dst and dst[0].get_device() != ts[0].get_device():
-            bad("gradients and outputs are on one GPU")
-        if ns != ons:
-            bad("an output has another number of elements than its gradient")
-        for t, o in zip(ts, dst):
-            if not (t.is_contiguous() and o.is_contiguous()) and t.stride() != o.stride():
-                bad("a gradient that is not contiguous needs an output of its own strides")
-        if any(o != d and o != _lib.F32 for o, d in zip(odts, dts)):
-            bad("an output is of its gradient's type or float32")
-    table = array.array("q", [v for row in zip(ptrs, outs, ns, [d | o << 32 for d, o in zip(dts, odts)]) for v in row])
+    dst = ts if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    table = array.array("q", bytes(32 * len(ts)))
+    bad = _lib.HOST.host_tensor_table(ts, dst, table.buffer_info()[0])
+    if bad is not None:
+        raise _lib.GanAmdError(f"{what}: {bad}")
     return ts, dst, table
 
 
@@ -1822,7 +1780,7 @@ def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=None, 
     if not max_norm >= 0:
         raise _lib.GanAmdError(f"clip_grad_norm_: max_norm {max_norm}")
     ts, dst, table = _tensor_list("clip_grad_norm_", tensors, out)
-    if any(t.requires_grad for t in dst):
+    if _lib.HOST.host_requires_grad(dst):
         raise _lib.GanAmdError("clip_grad_norm_: writes into a tensor that requires a gradient (detach it)")
     if not ts:
         return torch.zeros((), device="cuda")
