@@ -14,7 +14,6 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.environ.get("GANAMD_SO") or os.path.join(_HERE, "libganamd.so")   # GANAMD_SO: A/B builds
-HOST_PATH = os.path.join(_HERE, "libganamd_host.so")
 
 c_int = ctypes.c_int
 c_long = ctypes.c_long
@@ -189,23 +188,22 @@ def _load():
 LIB = _load()
 
 
+class GanAmdError(RuntimeError):
+    pass
+
+
 def _load_host():
-    """libganamd_host.so (csrc/host.cpp): reads lists of torch tensors, with the GIL held."""
-    if not os.path.exists(HOST_PATH):
-        raise ImportError(f"{HOST_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
-    lib = ctypes.PyDLL(HOST_PATH)
-    lib.host_tensor_table.restype = ctypes.py_object
-    lib.host_tensor_table.argtypes = [ctypes.py_object, ctypes.py_object, vp]
-    lib.host_requires_grad.restype = c_int
-    lib.host_requires_grad.argtypes = [ctypes.py_object]
-    return lib
+    """The module _host.so (csrc/host.cpp): autograd nodes and list reading of the operators whose
+    host side is native.  It calls LIB's entry points, handed over by address."""
+    try:
+        from . import _host
+    except ImportError as e:
+        raise ImportError(f"{_HERE}/_host.so: {e}; build it with `python -c 'import __graft_entry__ as g; g.build()'`") from e
+    _host.init(GanAmdError, {n: ctypes.cast(getattr(LIB, n), vp).value for n in _SIGS})
+    return _host
 
 
 HOST = _load_host()
-
-
-class GanAmdError(RuntimeError):
-    pass
 
 
 def check(rc: int, what: str):

@@ -369,30 +369,79 @@ __device__ __forceinline__ void accumulate(A (&acc)[K][NC], const Chan<MODE, ACT
   }
 }
 
-// Folds acc over the block's positions into chan[k * a.CT + slot] (LDS).  `sh`: scratch of
-// rows: P * CT values, planes: one per wave.  Every thread of the block calls it.
+// v of the lane that differs in bit `STEP` of its number, or of one whose value is the same once the
+// smaller steps are summed (a mirrored lane): DPP moves where there is one, half a dozen cycles
+// instead of an LDS permute's latency.
+template <int STEP>
+__device__ __forceinline__ uint32_t other(uint32_t v) {
+  if constexpr (STEP == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
+  else if constexpr (STEP == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+  else if constexpr (STEP == 4) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true);  // row_half_mirror
+  else if constexpr (STEP == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true);  // row_mirror
+  else return (uint32_t)__shfl_xor((int)v, STEP, 64);
+}
+template <int STEP>
+__device__ __forceinline__ float other(float v) { return __uint_as_float(other<STEP>(__float_as_uint(v))); }
+template <int STEP>
+__device__ __forceinline__ double other(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint64_t w = (uint64_t)other<STEP>((uint32_t)(u >> 32)) << 32 | other<STEP>((uint32_t)u);
+  return __builtin_bit_cast(double, w);
+}
+// The sum over W (a power of two, at most 64) neighbouring lanes, in each of them.
+template <class A>
+__device__ __forceinline__ A lanes_sum(A v, int W) {
+  if (W >= 2) v += other<1>(v);
+  if (W >= 4) v += other<2>(v);
+  if (W >= 8) v += other<4>(v);
+  if (W >= 16) v += other<8>(v);
+  if (W >= 32) v += other<16>(v);
+  if (W >= 64) v += other<32>(v);
+  return v;
+}
+
+// Sums that a round of a row tile's fold takes through LDS at once (32 KB of scratch).
+constexpr int fold_round(int K, int NC, int nt, int size) {
+  const int n = 32768 / (NC * nt * size);
+  return n < 1 ? 1 : n < K ? n : K;
+}
+
+// Folds acc over the block's positions into chan[k * a.CT + slot] (LDS), in one order.  `sh`: scratch
+// of rows: fold_round * NC * threads values (a thread's values nt apart: no bank conflicts), planes:
+// K * 16.  Every thread of the block calls it.
 template <bool ROWS, int V, int K, int NC, class A>
-__device__ __forceinline__ void fold(const Args& a, const Map<ROWS, V>& m, A (&acc)[K][NC], A* sh, A* chan) {
+__device__ __forceinline__ void fold(const Args& a, const Map<ROWS, V>& m, A (&acc)[K][NC], A* sh, A* chan, int c0) {
   const int tid = threadIdx.x, nt = blockDim.x;
   if constexpr (ROWS) {
-    int Q = 1;                                    // lanes that share a channel's fold
-    while (2 * Q * a.CT <= nt && 2 * Q <= a.P && Q < 64) Q *= 2;
-    for (int k = 0; k < K; ++k) {
+    const int R = fold_round(K, NC, nt, sizeof(A)), wid = min(a.CT, a.C - c0);
+    for (int k0 = 0; k0 < K; k0 += R) {
       __syncthreads();
-      if (m.active) {
 #pragma unroll
-        for (int j = 0; j < NC; ++j)
-          if (j >= m.skip0) sh[m.p * a.CT + m.slot + j] = acc[k][j];
-      }
+      for (int k = 0; k < K; ++k)
+        if (k >= k0 && k < k0 + R) {
+#pragma unroll
+          for (int j = 0; j < NC; ++j) sh[((k - k0) * NC + j) * nt + tid] = acc[k][j];
+        }
       __syncthreads();
-      const int q = tid & (Q - 1);
-      for (int c0 = 0; c0 < a.CT; c0 += nt / Q) {
-        const int c = c0 + tid / Q;
+      const int I = min(R, K - k0) * NC * a.TX, Q = max(1, min(nt / I, a.P));
+      for (int i0 = 0; i0 < I; i0 += nt) {                // one trip where Q > 1
+        const int i = i0 + tid % (Q > 1 ? I : nt), q = Q > 1 ? tid / I : 0;
+        const int tx = i % a.TX, kj = i / a.TX;
         A s = 0;
-        if (c < a.CT)
-          for (int p = q; p < a.P; p += Q) s += sh[p * a.CT + c];
-        for (int o = Q / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-        if (q == 0 && c < a.CT) chan[k * a.CT + c] = s;
+        if (i < I && q < Q) {
+          const A* p0 = sh + kj * nt + tx;
+#pragma unroll 4
+          for (int p = q; p < a.P; p += Q) s += p0[p * a.TX];
+        }
+        if (Q > 1) {
+          __syncthreads();
+          if (q < Q && q > 0) sh[(q - 1) * I + i] = s;
+          __syncthreads();
+          if (q == 0)
+            for (int o = 0; o < Q - 1; ++o) s += sh[o * I + i];
+        }
+        const int j = kj % NC, slot = max(min(tx * V, wid - V), -c0) + j;
+        if (q == 0 && i < I && tx * V < wid && slot >= tx * V) chan[(k0 + kj / NC) * a.CT + slot] = s;
       }
     }
     __syncthreads();
@@ -401,8 +450,7 @@ __device__ __forceinline__ void fold(const Args& a, const Map<ROWS, V>& m, A (&a
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      A s = m.active ? acc[k][0] : (A)0;
-      for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+      const A s = lanes_sum(m.active ? acc[k][0] : (A)0, lanes);
       if (nw == 1) {
         if (m.p == 0 && m.active) chan[k * a.CT + m.slot] = s;
       } else if ((tid & 63) == 0) {
@@ -422,12 +470,6 @@ __device__ __forceinline__ void fold(const Args& a, const Map<ROWS, V>& m, A (&a
       __syncthreads();
     }
   }
-}
-
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
 }
 
 // ------------------------------------------------------------------ group coefficients
@@ -633,25 +675,28 @@ __device__ __forceinline__ void load_lin(const Args& a, const Map<ROWS, V>& m, l
   }
 }
 
-// Groups c0 / Cg .. of sample b, a wave each, from their channels' sums chan[k * stride + c]:
-// statistics or coefficients to gco[8 a group], a sample's terms of the parameter gradients to par.
+// Groups c0 / Cg .. of sample b from their channels' sums chan[k * stride + c], W lanes each (the
+// channels of a group, at most a wave): statistics or coefficients to gco[8 a group], a sample's
+// terms of the parameter gradients to par.
 template <int MODE, int ACT, class A>
 __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int ng, const A* chan, long stride,
                                               double* gco) {
-  const int lane = threadIdx.x & 63, nw = blockDim.x >> 6, g0 = c0 / a.Cg;
+  int W = 1;
+  while (W < a.Cg && W < 64) W *= 2;
+  const int lane = threadIdx.x & (W - 1), g0 = c0 / a.Cg;
   const double invN = 1.0 / ((double)a.L * a.Cg);
-  for (int gi = threadIdx.x >> 6; gi < ng; gi += nw) {
+  for (int gi = threadIdx.x / W; gi < ng; gi += blockDim.x / W) {
     const int cg = gi * a.Cg;
     double* st = a.stats + 2 * (b * a.G + g0 + gi);
     double* co = gco + 8L * gi;
     if constexpr (MODE == FWD) {
       double s = 0, q = 0;
-      for (int c = lane; c < a.Cg; c += 64) {
+      for (int c = lane; c < a.Cg; c += W) {
         s += chan[cg + c];
         q += chan[stride + cg + c];
       }
-      s = wave_sum(s);
-      q = wave_sum(q);
+      s = lanes_sum(s, W);
+      q = lanes_sum(q, W);
       const double mean = s * invN, var = fmax(q * invN - mean * mean, 0.0);
       const double nan = s - s + (q - q);            // fmax drops a NaN: put it back
       const double r = 1.0 / sqrt(var + nan + (double)a.eps);
@@ -665,7 +710,7 @@ __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int
       const Group q = group_of(st[0], st[1]);
       const int cc = c0 + cg;
       double m1[4] = {0, 0, 0, 0};
-      for (int c = lane; c < a.Cg; c += 64) {
+      for (int c = lane; c < a.Cg; c += W) {
         double terms[3];
         sweep1<MODE, ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * stride + cg + c]; }, m1, terms);
         if (MODE == BWD && a.par)
@@ -673,7 +718,7 @@ __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int
           for (int k = 0; k < Sums<BWD, ACT>::K; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
       }
 #pragma unroll
-      for (int k = 0; k < (MODE == BWD ? 2 : 4); ++k) m1[k] = wave_sum(m1[k]) * invN;
+      for (int k = 0; k < (MODE == BWD ? 2 : 4); ++k) m1[k] = lanes_sum(m1[k], W) * invN;
       if (MODE == BWD) {
         if (lane == 0) {
           co[0] = m1[0];
@@ -681,7 +726,7 @@ __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int
         }
       } else {
         double m2[3] = {0, 0, 0};
-        for (int c = lane; c < a.Cg; c += 64) {
+        for (int c = lane; c < a.Cg; c += W) {
           double terms[3];
           sweep2<ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * stride + cg + c]; }, m1, m2, terms);
           if (a.par)
@@ -689,7 +734,7 @@ __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int
             for (int k = 0; k < 3; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
         }
 #pragma unroll
-        for (int k = 0; k < 3; ++k) m2[k] = wave_sum(m2[k]);
+        for (int k = 0; k < 3; ++k) m2[k] = lanes_sum(m2[k], W);
         if (lane == 0) dbl_coef(q, m1, m2, invN, co);
       }
     }
@@ -757,7 +802,7 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
     if constexpr (MODE >= BWD) gy[k].pin();
     if constexpr (MODE == DBL) v[k].pin();
   }
-  fold<ROWS, V, K, NC>(a, m, acc, sh, chan);
+  fold<ROWS, V, K, NC>(a, m, acc, sh, chan, c0);
   finish_groups<MODE, ACT>(a, b, c0, ng, chan, (long)a.CT, gco);
   __syncthreads();
   Lin<MODE, ACT> ln[NC];
@@ -778,6 +823,17 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
 }
 
 // ------------------------------------------------------------------ the split form
+#ifndef GN_US
+#define GN_US 4
+#define GN_UD 2
+#define GN_UA 2
+#endif
+#ifndef GN_PF
+#define GN_PF 1
+#endif
+#ifndef GN_BLOCKS
+#define GN_BLOCKS 512
+#endif
 constexpr int kNT = 512;
 
 // The loop of both passes over a chunk: U positions at a time, the next ones loaded before the
@@ -819,9 +875,10 @@ __device__ __forceinline__ void stream(const Args& a, const Map<ROWS, V>& m, int
       ca[u] = at[u];
       cs[u] = skip[u];
     }
-    if (i0 + step < hi) fetch(i0 + step);
+    if (GN_PF && i0 + step < hi) fetch(i0 + step);
 #pragma unroll
     for (int u = 0; u < U; ++u) use(ca[u], cs[u], cx[u], cg[MODE >= BWD ? u : 0], cv[MODE == DBL ? u : 0]);
+    if (!GN_PF && i0 + step < hi) fetch(i0 + step);
   }
 }
 
@@ -829,7 +886,7 @@ __device__ __forceinline__ void stream(const Args& a, const Map<ROWS, V>& m, int
 template <int MODE, int ACT, bool ROWS, class T, int V>
 __global__ __launch_bounds__(kNT) void sums_kernel(Args a) {
   typedef typename AccT<MODE>::type A;
-  constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K, U = MODE == DBL ? 2 : 4;
+  constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K, U = MODE == DBL ? GN_UD : GN_US;
   extern __shared__ __align__(16) char lds[];
   const int s = blockIdx.x % a.S, tile = blockIdx.x / a.S % a.nct;
   const int bi = blockIdx.x / a.S / a.nct;
@@ -854,7 +911,7 @@ __global__ __launch_bounds__(kNT) void sums_kernel(Args a) {
         if constexpr (MODE == DBL) v.zero_front(skip);
         accumulate<MODE, ACT, ROWS, T, V, NC>(acc, ch, x, gy, v);
       });
-  fold<ROWS, V, K, NC>(a, m, acc, sh, chan);
+  fold<ROWS, V, K, NC>(a, m, acc, sh, chan, c0);
   A* part = reinterpret_cast<A*>(a.part) + ((long)bi * a.S + s) * K * a.C;
   for (int i = threadIdx.x; i < K * wid; i += blockDim.x)
     part[(long)(i / wid) * a.C + c0 + i % wid] = chan[i / wid * a.CT + i % wid];
@@ -897,7 +954,7 @@ __global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) 
 #pragma unroll 8
         for (int s = q; s < ns; s += sw) t += (double)p[s * hop];
       }
-      for (int o = sw / 2; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+      t = lanes_sum(t, sw);
       if (q == 0 && i < pairs) *p = (A)t;
     }
     __syncthreads();
@@ -909,7 +966,7 @@ __global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) 
 
 template <int MODE, int ACT, bool ROWS, class T, int V>
 __global__ __launch_bounds__(kNT) void apply_kernel(Args a) {
-  constexpr int NC = ROWS ? V : 1, U = 2;
+  constexpr int NC = ROWS ? V : 1, U = GN_UA;
   extern __shared__ __align__(16) char lds[];
   const int s = blockIdx.x % a.S, tile = blockIdx.x / a.S % a.nct;
   const long b = a.b0 + blockIdx.x / a.S / a.nct;

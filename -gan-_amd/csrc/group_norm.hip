@@ -86,7 +86,7 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   if (p.resident) {
     a.S = 1;
     a.per = 0;
-    const size_t sh = p.rows ? (size_t)a.P * a.CT : (size_t)K * 16;
+    const size_t sh = p.rows ? (size_t)gn::fold_round(K, p.V, p.nt, asz) * p.V * p.nt : (size_t)K * 16;
     p.lds = (size_t)(a.CT / Cg) * 64 + std::max(asz * ((size_t)K * a.CT + sh), 4 * (size_t)tabs * a.CT);
     if (p.lds > 64 * 1024) p.resident = false;
   }
@@ -111,11 +111,19 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     }
     // four blocks of eight waves a CU, but four vectors a thread at least, and at most 128 values of
     // a channel in one thread's fp32 sums
-    long S = std::max<long>(1, std::min(up_to(1024, B * a.nct), up_to(npos, 4L * a.P)));
+#ifdef GN_SLICE
+    {
+      const long per_sample = (mode == gn::FWD ? 2 : mode == gn::BWD ? 3 : 5) * L * C * esz;
+      const long n = std::max<long>(1, (GN_SLICE * 1048576L) / per_sample);
+      if (n < B) p.slice = (int)up_to(B, up_to(B, n));
+    }
+#endif
+    const long nb = p.slice;
+    long S = std::max<long>(1, std::min(up_to(GN_BLOCKS, nb * a.nct), up_to(npos, 4L * a.P)));
     S = std::max(S, up_to(npos, (p.rows ? 128L : 128L / p.V) * a.P));
     a.per = (int)(up_to(up_to(npos, S), a.P) * a.P);
     a.S = (int)up_to(npos, a.per);
-    const size_t sh = p.rows ? (size_t)a.P * a.CT : (size_t)K * 16;
+    const size_t sh = p.rows ? (size_t)gn::fold_round(K, p.V, p.nt, asz) * p.V * p.nt : (size_t)K * 16;
     p.lds = std::max(asz * ((size_t)K * a.CT + sh), 4 * (size_t)tabs * a.CT);
     p.apply_lds = 4 * (size_t)tabs * a.CT;
   }

@@ -13,7 +13,6 @@ Generator-only operators (fused BatchNorm+PReLU, the modulated conv) are first-o
 """
 from __future__ import annotations
 
-import array
 import contextlib
 import os
 import weakref
@@ -1510,202 +1509,10 @@ def branch_share(*tensors):
 # group norm with its activation (twice differentiable: per-sample statistics, for critics too)
 # ------------------------------------------------------------------------------------------
 
-_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
-_NORM_ACTS = {"none": _lib.NORM_NONE, "silu": _lib.NORM_SILU, "leaky": _lib.NORM_LEAKY, "prelu": _lib.NORM_PRELU}
-_NORM_LAYOUTS = {"nhwc": _lib.NORM_ROWS, "cnhw": _lib.NORM_PLANES}
-_NORM_CACHE: dict = {}
-
-
-def _on(t):
-    """Launches go to ``t``'s device: a guard where that is not the current one."""
-    if t.get_device() == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
-
-
-def _dptr(t):
-    return None if t is None else t.data_ptr()
-
-
-class _NormCfg:
-    """One group norm's descriptor and workspace sizes (shapes and types only)."""
-
-    __slots__ = ("desc", "ws", "groups", "shape", "has_slope")
-
-    def __init__(self, x, groups, pdt, act, slope, eps, layout):
-        B, C = (x.shape[0], x.shape[-1]) if layout == "nhwc" else (x.shape[1], x.shape[0])
-        self.shape, self.groups, self.has_slope = (B, C), groups, act == "prelu"
-        L = x.numel() // (B * C) if x.numel() else 0
-        self.desc = _lib.NormDesc(L, B, C, groups, _NORM_LAYOUTS[layout], _DTYPES[x.dtype], _DTYPES[pdt],
-                                  _NORM_ACTS[act], float(slope) if act == "leaky" else 0.0, float(eps))
-        self.ws = [None, None, None]
-
-    def workspace(self, op, device):
-        n = self.ws[op]
-        if n is None:
-            v = _lib.c_size_t(0)
-            check(LIB.ganamd_group_norm_workspace(self.desc, op, v), "group_norm_workspace")
-            n = self.ws[op] = v.value
-        return workspace(n, device) if n else None
-
-
-def _norm_cfg(x, groups, weight, bias, act, slope, eps, layout):
-    pars = [t for t in (weight, bias, slope if act == "prelu" else None) if t is not None]
-    pdt = pars[0].dtype if pars else torch.float32
-    key = (x.shape, x.dtype, groups, pdt, act, slope if act == "leaky" else None, eps, layout)
-    cfg = _NORM_CACHE.get(key)
-    if cfg is None:
-        def bad(msg):
-            raise _lib.GanAmdError(f"group_norm_act: {msg}")
-        if act not in _NORM_ACTS:
-            bad(f"act {act!r} is none of {sorted(_NORM_ACTS)}")
-        if layout not in _NORM_LAYOUTS:
-            bad(f"layout {layout!r} is neither 'nhwc' nor 'cnhw'")
-        if x.dtype not in _DTYPES:
-            bad(f"x is {x.dtype}: float32, bfloat16 or float16")
-        if x.dim() < 2:
-            bad(f"x has shape {tuple(x.shape)}: a batch and a channel dimension at least")
-        C = x.shape[-1] if layout == "nhwc" else x.shape[0]
-        if not isinstance(groups, int) or groups < 1 or C < 1 or C % groups:
-            bad(f"{groups} groups do not divide {C} channels")
-        if pdt not in (torch.float32, x.dtype):
-            bad(f"parameters are {pdt}: float32 or x's type ({x.dtype})")
-        if act == "leaky" and not isinstance(slope, (int, float)):
-            bad("act='leaky' takes a number as its slope")
-        if act in ("none", "silu") and slope is not None:
-            bad(f"act={act!r} takes no slope")
-        if not eps > 0:
-            bad(f"eps {eps}: more than 0")
-        if len(_NORM_CACHE) >= 4096:
-            _NORM_CACHE.clear()
-        cfg = _NORM_CACHE[key] = _NormCfg(x, groups, pdt, act, slope, eps, layout)
-    C = cfg.shape[1]
-    if act == "prelu" and not isinstance(slope, torch.Tensor):
-        raise _lib.GanAmdError("group_norm_act: act='prelu' takes a tensor of slopes, one per channel")
-    if not x.is_cuda:
-        raise _lib.GanAmdError(f"group_norm_act: x is on {x.device}")
-    for t in pars:
-        if t.dtype != pdt or t.numel() != C or t.device != x.device:
-            raise _lib.GanAmdError(f"group_norm_act: parameters are {C} elements of one type on x's device; "
-                                   f"got {tuple(t.shape)} {t.dtype} {t.device}")
-    return cfg
-
-
-def _norm_forward(cfg, x, w, b, slope):
-    y = torch.empty_like(x)
-    B, _ = cfg.shape
-    stats = torch.empty((B, cfg.groups, 2), device=x.device, dtype=torch.float64)
-    if x.numel():
-        with _on(x):
-            check(LIB.ganamd_group_norm_fwd(cfg.desc, x.data_ptr(), _dptr(w), _dptr(b), _dptr(slope), y.data_ptr(),
-                                            stats.data_ptr(), *wsarg(cfg.workspace(0, x.device)), stream()),
-                  "group_norm_fwd")
-    return y, stats
-
-
-def _norm_backward(cfg, gy, x, w, b, slope, stats, gx, gw, gb, gs, accumulate):
-    if not x.numel():
-        for t in (gw, gb, gs):
-            if t is not None and not accumulate:
-                t.zero_()
-        return
-    with _on(x):
-        check(LIB.ganamd_group_norm_bwd(cfg.desc, gy.data_ptr(), x.data_ptr(), _dptr(w), _dptr(b), _dptr(slope),
-                                        stats.data_ptr(), _dptr(gx), _dptr(gw), _dptr(gb), _dptr(gs), int(accumulate),
-                                        *wsarg(cfg.workspace(1, x.device)), stream()), "group_norm_bwd")
-
-
-def _in_flat(p) -> bool:
-    return p is not None and getattr(p if p._base is None else p._base, "_gan_flat", None) is not None
-
-
-def _norm_wants(args, need):
-    """Which parameter gradients a norm's backward makes.  One of a flat-buffer parameter is added to
-    that buffer, so it is only made where the engine asks for it (``wanted``; elsewhere a gradient
-    nobody asked for is dropped by the engine, which costs less than asking)."""
-    return [n and (not _in_flat(a) or wanted(a)) for n, a in zip(need, args)]
-
-
-def _param_targets(args, pars, need):
-    """Where the gradients of a norm's parameters go: (buffers, accumulate) -- the flat gradient
-    buffers when all wanted ones live there, new tensors otherwise (None: not wanted)."""
-    need = _norm_wants(args, need)
-    flat = [flat_grad(a) if n else None for n, a in zip(need, args)]
-    if any(need) and all(f is not None for n, f in zip(need, flat) if n) and all(
-            f.dtype == torch.float32 == p.dtype for f, p in zip(flat, pars) if f is not None):
-        return flat, True
-    return [torch.empty_like(p) if n else None for n, p in zip(need, pars)], False
-
-
-class GroupNormAct(Function):
-    """y = act(group_norm(x) * w + b); see ``group_norm_act``, which makes every input contiguous (a
-    copy made here would be saved without its history: no second derivative by x)."""
-
-    @staticmethod
-    def forward(ctx, x, w, b, slope, cfg):
-        ctx.args, ctx.cfg = (w, b, slope), cfg
-        y, stats = _norm_forward(cfg, x, w, b, slope)
-        ctx.save_for_backward(x, w, b, slope, stats)
-        return y
-
-    @staticmethod
-    def backward(ctx, gy):
-        x, w, b, slope, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        if torch.is_grad_enabled():                       # create_graph: differentiable once more
-            want = _norm_wants(ctx.args, need[1:4])
-            return (*GroupNormActBackward.apply(gy, x, *ctx.args, stats, ctx.cfg, want), None)
-        gy = _c(gy)
-        gx = torch.empty_like(x) if need[0] else None
-        (gw, gb, gs), acc = _param_targets(ctx.args, (w, b, slope), need[1:4])
-        _norm_backward(ctx.cfg, gy, x, w, b, slope, stats, gx, gw, gb, gs, acc)
-        return (gx, None, None, None, None) if acc else (gx, gw, gb, gs, None)
-
-
-class GroupNormActBackward(Function):
-    """(gx, gw, gb, gslope) of GroupNormAct as functions of (gy, x, w, b, slope): their own backward
-    is one reduction and one elementwise pass (ganamd_group_norm_bwd_bwd)."""
-
-    @staticmethod
-    def forward(ctx, gy, x, w, b, slope, stats, cfg, want):
-        ctx.set_materialize_grads(False)
-        ctx.args, ctx.cfg = (w, b, slope), cfg
-        gy = _c(gy)
-        gx = torch.empty_like(x)
-        g = [torch.empty_like(p) if n else None for n, p in zip(want, (w, b, slope))]
-        _norm_backward(cfg, gy, x, w, b, slope, stats, gx, *g, False)
-        ctx.save_for_backward(gy, x, w, b, slope, stats)
-        return (gx, *g)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, ggx, ggw, ggb, ggs):
-        gy, x, w, b, slope, stats = ctx.saved_tensors
-        cfg, need = ctx.cfg, ctx.needs_input_grad
-        if ggx is None and ggw is None and ggb is None and ggs is None:
-            return (None,) * 8
-        ggx = torch.zeros_like(x) if ggx is None else _c(ggx)
-        ggw, ggb, ggs = (None if t is None else _c(t) for t in (ggw, ggb, ggs))
-        (gw, gb, gs), acc = _param_targets(ctx.args, (w, b, slope), need[2:5])
-        g_gy, g_x = torch.empty_like(x), torch.empty_like(x)
-        if x.numel():
-            with _on(x):
-                check(LIB.ganamd_group_norm_bwd_bwd(
-                    cfg.desc, ggx.data_ptr(), _dptr(ggw), _dptr(ggb), _dptr(ggs), gy.data_ptr(), x.data_ptr(),
-                    _dptr(w), _dptr(b), _dptr(slope), stats.data_ptr(), g_gy.data_ptr(), g_x.data_ptr(), _dptr(gw),
-                    _dptr(gb), _dptr(gs), int(acc), *wsarg(cfg.workspace(2, x.device)), stream()),
-                    "group_norm_bwd_bwd")
-        elif not acc:
-            for t in (gw, gb, gs):
-                if t is not None:
-                    t.zero_()
-        par = (None, None, None) if acc else (gw, gb, gs)
-        return (g_gy if need[0] else None, g_x if need[1] else None, *par, None, None, None)
-
 
 def group_norm_act(x, groups: int, weight=None, bias=None, act: str = "none", slope=None, eps: float = 1e-5,
                    layout: str = "nhwc"):
-    """``act(group_norm(x) * weight + bias)`` as one operator, any order of derivative up to the second
+    """``act(group_norm(x) * weight + bias)`` as one operator, differentiable twice
     (``autograd.grad(create_graph=True)`` and a backward through it: the gradient penalty).
 
     ``x``: float32, bfloat16 or float16, channels last ``[B, ..., C]`` (``layout="nhwc"``; a torch
@@ -1714,15 +1521,10 @@ def group_norm_act(x, groups: int, weight=None, bias=None, act: str = "none", sl
     normalised by its own mean and biased variance (+ ``eps``).  ``weight`` / ``bias``: ``[C]`` or
     None (ones / zeros).  ``act``: ``"none"``, ``"silu"``, ``"leaky"`` (``slope``: a number; 0 is a
     ReLU), ``"prelu"`` (``slope``: ``[C]``, with a gradient).  Parameters are all float32 or all of
-    x's type, as are their gradients; the arithmetic is float32, statistics float64.
+    x's type, as are their gradients; the arithmetic is float32, statistics float64.  Gradients of
+    parameters in an optimizer's flat buffer are added there by the kernel.
     A non-contiguous ``x`` is copied first; an empty one gives an empty result."""
-    cfg = _norm_cfg(x, groups, weight, bias, act, slope, eps, layout)
-    x = _c(x)
-    weight, bias, slope = (None if t is None else _c(t) for t in (weight, bias, slope if cfg.has_slope else None))
-    if torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad
-                                                           for t in (weight, bias, slope))):
-        return GroupNormAct.apply(x, weight, bias, slope, cfg)
-    return _norm_forward(cfg, x, weight, bias, slope)[0]
+    return _lib.HOST.group_norm_act(x, groups, weight, bias, act, slope, eps, layout)
 
 
 # ------------------------------------------------------------------------------------------
@@ -1732,22 +1534,15 @@ def group_norm_act(x, groups: int, weight=None, bias=None, act: str = "none", sl
 _NORM_KINDS = {2.0: _lib.NORM_L2, float("inf"): _lib.NORM_MAX}
 
 
-def _tensor_list(what, tensors, out=None):
-    """The host table of a list of gradients (ganamd_tensor rows), checked (csrc/host.cpp)."""
-    ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    dst = ts if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
-    table = array.array("q", bytes(32 * len(ts)))
-    bad = _lib.HOST.host_tensor_table(ts, dst, table.buffer_info()[0])
-    if bad is not None:
-        raise _lib.GanAmdError(f"{what}: {bad}")
-    return ts, dst, table
-
-
 def _norm_kind(what, norm_type):
     try:
         return _NORM_KINDS[float(norm_type)]
     except KeyError:
         raise _lib.GanAmdError(f"{what}: norm_type {norm_type} is neither 2 nor inf") from None
+
+
+def _as_list(tensors):
+    return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
 
 
 def grad_norm(tensors, norm_type: float = 2.0):
@@ -1756,15 +1551,8 @@ def grad_norm(tensors, norm_type: float = 2.0):
     infinity the largest magnitude.  Tensors of any number, size (empty ones included) and of mixed
     types; densely stored."""
     kind = _norm_kind("grad_norm", norm_type)
-    ts, _, table = _tensor_list("grad_norm", tensors)
-    if not ts:
-        return torch.zeros((), device="cuda")
-    with _on(ts[0]):
-        norm = torch.empty((), device=ts[0].device, dtype=torch.float32)
-        at = table.buffer_info()[0]
-        ws = workspace(LIB.ganamd_grad_norm_workspace(at, len(ts)), norm.device)
-        check(LIB.ganamd_grad_norm(at, len(ts), kind, norm.data_ptr(), *wsarg(ws), stream()), "grad_norm")
-    return norm
+    ts = _as_list(tensors)
+    return _lib.HOST.grad_norm(ts, kind) if ts else torch.zeros((), device="cuda")
 
 
 def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=None, error_if_nonfinite: bool = False):
@@ -1779,26 +1567,17 @@ def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=None, 
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise _lib.GanAmdError(f"clip_grad_norm_: max_norm {max_norm}")
-    ts, dst, table = _tensor_list("clip_grad_norm_", tensors, out)
-    if _lib.HOST.host_requires_grad(dst):
-        raise _lib.GanAmdError("clip_grad_norm_: writes into a tensor that requires a gradient (detach it)")
-    if not ts:
+    ts = _as_list(tensors)
+    dst = None if out is None else _as_list(out)
+    if not ts and not dst:
         return torch.zeros((), device="cuda")
-    with _on(ts[0]):
-        if error_if_nonfinite:
-            if _lib.capture_id():
-                raise _lib.GanAmdError("clip_grad_norm_: error_if_nonfinite inside a graph capture")
-            n = float(grad_norm(ts, norm_type))
-            if n != n or n == float("inf"):
-                raise _lib.GanAmdError(f"clip_grad_norm_: the norm of the gradients is {n}")
-        norm = torch.empty((), device=ts[0].device, dtype=torch.float32)
-        at = table.buffer_info()[0]
-        ws = workspace(LIB.ganamd_grad_norm_workspace(at, len(ts)), norm.device)
-        rc = LIB.ganamd_grad_clip(at, len(ts), kind, max_norm, norm.data_ptr(), *wsarg(ws), stream())
-        if rc == -1:
-            raise _lib.GanAmdError("clip_grad_norm_: tensors that are written to share memory with others of the call")
-        check(rc, "grad_clip")
-    return norm
+    if error_if_nonfinite:
+        if _lib.capture_id():
+            raise _lib.GanAmdError("clip_grad_norm_: error_if_nonfinite inside a graph capture")
+        n = float(grad_norm(ts, norm_type))
+        if n != n or n == float("inf"):
+            raise _lib.GanAmdError(f"clip_grad_norm_: the norm of the gradients is {n}")
+    return _lib.HOST.clip(ts, dst, max_norm, kind)
 
 
 def clipped_adamw_(param, grad, exp_avg, exp_avg_sq, step, lr, betas, eps, weight_decay, max_norm, norm=None):
@@ -1806,26 +1585,4 @@ def clipped_adamw_(param, grad, exp_avg, exp_avg_sq, step, lr, betas, eps, weigh
     norm ``max_norm``: ``param``, ``exp_avg``, ``exp_avg_sq`` and the int32 device counter ``step``
     are updated in place, ``grad`` stays unscaled.  Returns the norm (0-dim float32 on the device;
     ``norm``: a tensor to write it into).  Two launches, no host synchronisation."""
-    n = param.numel()
-    bufs = (param, grad, exp_avg, exp_avg_sq)
-    for t, nm in zip(bufs, ("param", "grad", "exp_avg", "exp_avg_sq")):
-        _need(t, n, f"clipped_adamw_ {nm}")
-    _need(step, 1, "clipped_adamw_ step")
-    _need(norm, 1, "clipped_adamw_ norm")
-    if not float(max_norm) >= 0:
-        raise _lib.GanAmdError(f"clipped_adamw_: max_norm {max_norm}")
-    ptrs = [ptr(t) for t in bufs]
-    if len({t.device for t in bufs} | {step.device}) > 1 or any(abs(a - b) < 4 * n for i, a in enumerate(ptrs) for b in ptrs[:i]):
-        raise _lib.GanAmdError("clipped_adamw_: four separate buffers and the counter, on one device")
-    with _on(param):
-        if norm is None:
-            norm = torch.empty((), device=param.device, dtype=torch.float32)
-        if n:
-            ws = workspace(LIB.ganamd_adamw_clip_workspace(), param.device)
-            check(LIB.ganamd_adamw_clip(*ptrs, n, iptr(step), float(lr), float(betas[0]), float(betas[1]), float(eps),
-                                        float(weight_decay), float(max_norm), ptr(norm), *wsarg(ws), stream()),
-                  "adamw_clip")
-        else:
-            norm.zero_()
-            step.add_(1)
-    return norm
+    return _lib.HOST.clipped_adamw(param, grad, exp_avg, exp_avg_sq, step, lr, *betas, eps, weight_decay, max_norm, norm)

@@ -86,10 +86,10 @@ def test_formulas_match_differences(act):
 # ------------------------------------------------------------------ plans
 
 def plan(shape, G, dtype, act, layout, op):
-    from gan_amd import _lib, ops
+    from gan_amd import _lib
     B, C = (shape[0], shape[-1]) if layout == "nhwc" else (shape[1], shape[0])
-    d = _lib.NormDesc(math.prod(shape) // (B * C), B, C, G, ops._NORM_LAYOUTS[layout], ops._DTYPES[dtype], 0,
-                      ops._NORM_ACTS[act], 0.2, 1e-5)
+    d = _lib.NormDesc(math.prod(shape) // (B * C), B, C, G, ("nhwc", "cnhw").index(layout),
+                      (torch.float32, torch.bfloat16, torch.float16).index(dtype), 0, ACTS.index(act), 0.2, 1e-5)
     info, n = (ctypes.c_int * 10)(), _lib.c_size_t(0)
     assert _lib.LIB.ganamd_group_norm_plan_info(d, op, info) == 0
     assert _lib.LIB.ganamd_group_norm_workspace(d, op, n) == 0

@@ -320,6 +320,16 @@ def test_penalty_step_with_group_norm_and_clip(act):
             assert float((u.detach().double().cpu() - q[k].detach()).abs().max()) < 4e-4 * 1e-3 + 2.0 ** -22, k
 
 
+def test_group_norm_third_derivative_is_refused(ops):
+    t = make((2, 4, 8), "nhwc", "silu", F32, 19)
+    x, gy = (t[k].detach().requires_grad_() for k in ("x", "gy"))
+    y = ops.group_norm_act(x, 2, t["w"], t["b"], act="silu")
+    (gx,) = torch.autograd.grad(y, x, gy, create_graph=True)
+    (g2,) = torch.autograd.grad(gx, x, t["v"], create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g2.sum().backward()
+
+
 def test_group_norm_flat_gradients(ops):
     """Gradients of parameters in an optimizer's flat buffer are added there, and only when asked."""
     from gan_amd.optim import FusedAdamW
@@ -338,6 +348,20 @@ def test_group_norm_flat_gradients(ops):
     for p, g in zip((D.gamma, D.beta, D.slope), want):
         assert torch.equal(p.grad, g + g)
         assert p.grad.data_ptr() >= D._flat.grad.data_ptr()
+    # asked for by autograd.grad, they are returned and the buffer stays as it is
+    keep = D._flat.grad.clone()
+    for p, g, u in zip((D.gamma, D.beta, D.slope), want, torch.autograd.grad(call(t["x"]), (D.gamma, D.beta, D.slope), t["gy"])):
+        assert torch.equal(g, u)
+    assert torch.equal(keep, D._flat.grad)
+    # through the penalty: the second backward adds them to the buffer
+    D._flat.grad.zero_()
+    (gx,) = torch.autograd.grad(call(x), x, t["gy"], create_graph=True)
+    assert not D._flat.grad.any()
+    gx.backward(t["v"])
+    y = ops.group_norm_act(x, 2, free[0], free[1], act="prelu", slope=free[2], layout="cnhw")
+    (gx,) = torch.autograd.grad(y, x, t["gy"], create_graph=True)
+    for p, g in zip((D.gamma, D.slope), torch.autograd.grad(gx, (free[0], free[2]), t["v"])):
+        assert torch.equal(p.grad, g)
 
 
 def test_group_norm_graph(ops):
