@@ -4,9 +4,10 @@
 //   n = sqrt(sum_k sum_i g_ki^2)  (or max |g_ki|),  c = min(1, max_norm / (n + 1e-6)),  g <- c g
 //
 // What bounds them: memory (clip: one read, one read + write of every gradient; step: 4 + 28 bytes
-// a parameter).  The tensors are cut into chunks, one block each.  A launch carries its table of
-// tensors in its arguments, so a call needs no copy to the device and can be captured; more tensors
-// than a table holds take more launches.  Squares are summed in 64 bits: no gradient of a finite
+// a parameter).  The tensors are cut into chunks, one block each.  The table of tensors travels in
+// launch arguments, so a call needs no copy to the device and can be captured: one that fits the
+// arguments is read there; a longer one is laid out in the workspace by small launches first, which
+// costs less than a norm and a scaling launch for each piece of the list.  Squares are summed in 64 bits: no gradient of a finite
 // norm overflows or vanishes, and the order is fixed (no atomics).  The launch that scales folds
 // the chunks' partials itself, in every block alike, so a clip is two launches.
 
@@ -15,6 +16,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/ganamd.h"
 
@@ -24,6 +26,7 @@ constexpr int kNT = 256;
 constexpr long kChunkMin = 4096, kChunkMax = 16384;
 constexpr int kFoldMax = 1024;      // partials that every scaling block folds by itself
 constexpr int kTable = 160;         // tensors of a launch (the arguments stay under 4 KB)
+constexpr int kStepVec = 4;         // vectors of each buffer a thread of the step takes
 constexpr int kStepBlocks = 1024;   // partials of the flat buffer's norm
 
 struct Entry {
@@ -33,7 +36,15 @@ struct Entry {
 struct Table {
   Entry e[kTable];
   int n, chunk;         // tensors; elements per chunk
-  uint32_t chunks, base;// chunks of this launch; of the launches before it
+  uint32_t chunks;      // of this launch
+  uint32_t base, index; // chunks and tensors of the launches before it
+};
+// The same laid out in the workspace: a chunk's tensor, and the tensors (their chunks numbered through).
+struct Listed {
+  const Entry* e;
+  const uint32_t* owner;
+  int n, chunk;
+  uint32_t chunks;
 };
 
 __device__ __forceinline__ float bf(uint32_t h) { return __uint_as_float(h << 16); }
@@ -123,43 +134,60 @@ __device__ __forceinline__ void norm_chunk(const void* in, long lo, long n, Acc<
   for (long i = nv * V + threadIdx.x; i < n; i += kNT) acc.add(conv<DT>(p[i]));
 }
 
-// The tensor that holds this block's chunk: the lanes count the first chunks at or before it.
-__device__ __forceinline__ int find(const Table& t, uint32_t chunk) {
+// The piece of a tensor that this block's chunk is.
+struct Piece {
+  uint64_t in, out;
+  long lo, n;
+};
+
+__device__ __forceinline__ Piece piece(const Entry& e, uint32_t end, uint32_t chunk, int size) {
+  return {e.in, e.out, (long)(chunk - e.first) * size, chunk + 1 == end ? (long)e.tail : (long)size};
+}
+// in the arguments: the lanes count the tensors that start at or before the chunk
+__device__ __forceinline__ Piece find(const Table& t, uint32_t chunk) {
   int k = 0;
   for (int i = threadIdx.x & 63; i < kTable; i += 64) {
     const bool le = i < t.n && t.e[i].first <= chunk;
     k += __popcll(__ballot(le));
   }
-  return __builtin_amdgcn_readfirstlane(k) - 1;
+  k = __builtin_amdgcn_readfirstlane(k) - 1;
+  return piece(t.e[k], k + 1 < t.n ? t.e[k + 1].first : t.chunks, chunk, t.chunk);
+}
+__device__ __forceinline__ Piece find(const Listed& t, uint32_t chunk) {
+  const int k = (int)t.owner[chunk];
+  return piece(t.e[k], k + 1 < t.n ? t.e[k + 1].first : t.chunks, chunk, t.chunk);
 }
 
-__device__ __forceinline__ void span(const Table& t, int k, uint32_t chunk, long& lo, long& n) {
-  const uint32_t end = k + 1 < t.n ? t.e[k + 1].first : t.chunks;
-  lo = (long)(chunk - t.e[k].first) * t.chunk;
-  n = chunk + 1 == end ? t.e[k].tail : t.chunk;
+// Lays a launch's table out in the workspace, a block per tensor.
+__global__ __launch_bounds__(kNT) void list_kernel(Table t, Entry* e, uint32_t* owner) {
+  const int k = blockIdx.x;
+  const uint32_t first = t.e[k].first, end = k + 1 < t.n ? t.e[k + 1].first : t.chunks;
+  if (threadIdx.x == 0) {
+    Entry o = t.e[k];
+    o.first += t.base;
+    e[t.index + k] = o;
+  }
+  for (uint32_t c = first + threadIdx.x; c < end; c += kNT) owner[t.base + c] = t.index + k;
 }
 
 constexpr uint64_t kAddr = (1ull << 60) - 1;
 
-template <int KIND>
-__global__ __launch_bounds__(kNT) void norm_kernel(Table t, double* __restrict__ part) {
+template <int KIND, class Tab>
+__global__ __launch_bounds__(kNT) void norm_kernel(Tab t, double* __restrict__ part) {
   __shared__ double sh[kNT / 64];
   const uint32_t chunk = blockIdx.x;
-  const int k = find(t, chunk);
-  long lo, n;
-  span(t, k, chunk, lo, n);
-  const uint64_t e = t.e[k].in;
-  const void* in = reinterpret_cast<const void*>(e & kAddr);
-  const int dt = (int)(e >> 60);
+  const Piece q = find(t, chunk);
+  const void* in = reinterpret_cast<const void*>(q.in & kAddr);
+  const int dt = (int)(q.in >> 60);
   Acc<KIND> acc;
   if (dt == GANAMD_F32)
-    norm_chunk<KIND, GANAMD_F32>(in, lo, n, acc);
+    norm_chunk<KIND, GANAMD_F32>(in, q.lo, q.n, acc);
   else if (dt == GANAMD_BF16)
-    norm_chunk<KIND, GANAMD_BF16>(in, lo, n, acc);
+    norm_chunk<KIND, GANAMD_BF16>(in, q.lo, q.n, acc);
   else
-    norm_chunk<KIND, GANAMD_F16>(in, lo, n, acc);
+    norm_chunk<KIND, GANAMD_F16>(in, q.lo, q.n, acc);
   const double v = block_join<KIND, kNT>(acc, sh);
-  if (threadIdx.x == 0) part[t.base + chunk] = v;
+  if (threadIdx.x == 0) part[chunk] = v;
 }
 
 template <int KIND, int NT>
@@ -224,33 +252,30 @@ __device__ __forceinline__ void scale_chunk(const void* in, void* out, long lo, 
   for (long i = nv * V + threadIdx.x; i < n; i += kNT) q[i] = (SO)pack1<DO>(conv<DI>(p[i]) * c);
 }
 
-// n > 0: folds the partials itself; n == 0: part[0] is the norm.  The first block of all says it.
-template <int KIND>
-__global__ __launch_bounds__(kNT) void scale_kernel(Table t, const double* __restrict__ part, int n, float max_norm,
+// n > 0: folds the partials itself; n == 0: part[0] is the norm.  The first block says it.
+template <int KIND, class Tab>
+__global__ __launch_bounds__(kNT) void scale_kernel(Tab t, const double* __restrict__ part, int n, float max_norm,
                                                     float* norm) {
   __shared__ double sh[kNT / 64];
   const uint32_t chunk = blockIdx.x;
+  const Piece q = find(t, chunk);
   const double v = n > 0 ? fold<KIND, kNT>(part, n, sh) : part[0];
-  if (norm && chunk == 0 && t.base == 0 && threadIdx.x == 0) *norm = (float)v;
+  if (norm && chunk == 0 && threadIdx.x == 0) *norm = (float)v;
   const float c = clip_factor(v, max_norm);
-  const int k = find(t, chunk);
-  const uint64_t ei = t.e[k].in, eo = t.e[k].out;
-  if (c == 1.f && ei == eo) return;           // in place, times one
-  long lo, len;
-  span(t, k, chunk, lo, len);
-  const void* in = reinterpret_cast<const void*>(ei & kAddr);
-  void* out = reinterpret_cast<void*>(eo & kAddr);
-  const int di = (int)(ei >> 60), dn = (int)(eo >> 60);
+  if (c == 1.f && q.in == q.out) return;           // in place, times one
+  const void* in = reinterpret_cast<const void*>(q.in & kAddr);
+  void* out = reinterpret_cast<void*>(q.out & kAddr);
+  const int di = (int)(q.in >> 60), dn = (int)(q.out >> 60);
   if (di == GANAMD_F32)
-    scale_chunk<GANAMD_F32, GANAMD_F32>(in, out, lo, len, c);
+    scale_chunk<GANAMD_F32, GANAMD_F32>(in, out, q.lo, q.n, c);
   else if (di == GANAMD_BF16 && dn == GANAMD_BF16)
-    scale_chunk<GANAMD_BF16, GANAMD_BF16>(in, out, lo, len, c);
+    scale_chunk<GANAMD_BF16, GANAMD_BF16>(in, out, q.lo, q.n, c);
   else if (di == GANAMD_BF16)
-    scale_chunk<GANAMD_BF16, GANAMD_F32>(in, out, lo, len, c);
+    scale_chunk<GANAMD_BF16, GANAMD_F32>(in, out, q.lo, q.n, c);
   else if (dn == GANAMD_F16)
-    scale_chunk<GANAMD_F16, GANAMD_F16>(in, out, lo, len, c);
+    scale_chunk<GANAMD_F16, GANAMD_F16>(in, out, q.lo, q.n, c);
   else
-    scale_chunk<GANAMD_F16, GANAMD_F32>(in, out, lo, len, c);
+    scale_chunk<GANAMD_F16, GANAMD_F32>(in, out, q.lo, q.n, c);
 }
 
 // ------------------------------------------------------------------ the flat buffer's step
@@ -268,6 +293,10 @@ __global__ __launch_bounds__(kNT) void flat_norm_kernel(const float* __restrict_
   }
 }
 
+struct AdamArgs {
+  double lr, beta1, beta2, eps, wd;
+  float max_norm;
+};
 struct AdamConst {
   float c, size, root, decay, w, b2, omb2, eps;
 };
@@ -282,32 +311,34 @@ __device__ __forceinline__ void adamw_one(const AdamConst& k, float gi, float& p
   v = vi;
 }
 
+// A block takes kStepVec vectors a thread, one piece of each buffer: pieces go in launch order, so
+// what is in flight stays close together in memory (362 M parameters: 2.16 ms, 5.4 TB/s; blocks that
+// stride through the whole buffers: 2.58 ms; one vector a thread: 2.22).  Every block folds the
+// partials of the norm itself: a kernel of its own for that measured the same and is a launch more.
 __global__ __launch_bounds__(kNT) void adamw_clip_kernel(float* __restrict__ p, const float* __restrict__ g,
                                                          float* __restrict__ m, float* __restrict__ v, long n,
                                                          const double* __restrict__ part, int parts,
-                                                         const int32_t* __restrict__ step, double lr, double beta1,
-                                                         double beta2, double eps, double wd, float max_norm,
-                                                         float* norm) {
+                                                         const int32_t* __restrict__ step, AdamArgs a, float* norm) {
   __shared__ double sh[kNT / 64];
   __shared__ AdamConst ks;
   const double nv = fold<0, kNT>(part, parts, sh);
   if (threadIdx.x == 0) {
     const double t = (double)*step;
-    ks.c = clip_factor(nv, max_norm);
-    ks.size = (float)(lr / (1.0 - pow(beta1, t)));
-    ks.root = (float)sqrt(1.0 - pow(beta2, t));
-    ks.decay = (float)(1.0 - lr * wd);
-    ks.w = (float)(1.0 - beta1);
-    ks.b2 = (float)beta2;
-    ks.omb2 = (float)(1.0 - beta2);      // (of the 64-bit beta2: 1 - 0.999f is 1.3e-5 off 0.001)
-    ks.eps = (float)eps;
+    ks.c = clip_factor(nv, a.max_norm);
+    ks.size = (float)(a.lr / (1.0 - pow(a.beta1, t)));
+    ks.root = (float)sqrt(1.0 - pow(a.beta2, t));
+    ks.decay = (float)(1.0 - a.lr * a.wd);
+    ks.w = (float)(1.0 - a.beta1);
+    ks.b2 = (float)a.beta2;
+    ks.omb2 = (float)(1.0 - a.beta2);    // (of the 64-bit beta2: 1 - 0.999f is 1.3e-5 off 0.001)
+    ks.eps = (float)a.eps;
     if (blockIdx.x == 0) *norm = (float)nv;
   }
   __syncthreads();
   const AdamConst k = ks;
   typedef W16<4>::type W;
-  const long quads = n / 4, stride = (long)gridDim.x * kNT;
-  for (long i = blockIdx.x * (long)kNT + threadIdx.x; i < quads; i += stride) {
+  const long quads = n / 4, lo = blockIdx.x * (long)(kNT * kStepVec), hi = min(quads, lo + kNT * kStepVec);
+  for (long i = lo + threadIdx.x; i < hi; i += kNT) {
     const u32x4 gw = *reinterpret_cast<const W*>(g + 4 * i);
     u32x4 pw = *reinterpret_cast<const W*>(p + 4 * i), mw = *reinterpret_cast<const W*>(m + 4 * i),
           vw = *reinterpret_cast<const W*>(v + 4 * i);
@@ -334,19 +365,32 @@ inline int ok(hipError_t e) { return e == hipSuccess ? GANAMD_OK : GANAMD_ELAUNC
 inline long esize(int dt) { return dt == GANAMD_F32 ? 4 : 2; }
 inline bool is_type(int dt) { return dt >= GANAMD_F32 && dt <= GANAMD_F16; }
 
-// Elements per chunk (about 2048 chunks, a power of two) and the chunks of the whole list; -1: bad list.
-long plan(const ganamd_tensor* l, int n, long& chunk) {
-  if (n < 0 || (n && !l)) return -1;
+// How a list is cut: elements per chunk (about 2048 chunks, a power of two between 4 K and 16 K
+// elements: a block's work and 32 KB to 64 KB in flight) and where things lie in the workspace.
+struct Plan {
+  long chunk, chunks;
+  int tensors;                        // with elements
+  size_t entries, owner, total;       // behind the partials and the folded norm; total bytes
+};
+
+bool plan(const ganamd_tensor* l, int n, Plan& p) {
+  if (n < 0 || (n && !l)) return false;
   long total = 0;
+  p.tensors = 0;
   for (int i = 0; i < n; ++i) {
-    if (l[i].n < 0 || l[i].n > (1L << 40) || !is_type(l[i].dtype) || (l[i].n && !l[i].p)) return -1;
+    if (l[i].n < 0 || l[i].n > (1L << 40) || !is_type(l[i].dtype) || (l[i].n && !l[i].p)) return false;
     total += l[i].n;
+    p.tensors += l[i].n > 0;
   }
-  chunk = kChunkMin;
-  while (chunk < kChunkMax && total / chunk > 2048) chunk *= 2;
-  long chunks = 0;
-  for (int i = 0; i < n; ++i) chunks += (l[i].n + chunk - 1) / chunk;
-  return chunks < (1L << 31) ? chunks : -1;
+  p.chunk = kChunkMin;
+  while (p.chunk < kChunkMax && total / p.chunk > 2048) p.chunk *= 2;
+  p.chunks = 0;
+  for (int i = 0; i < n; ++i) p.chunks += (l[i].n + p.chunk - 1) / p.chunk;
+  if (p.chunks >= (1L << 31)) return false;
+  p.entries = sizeof(double) * ((size_t)p.chunks + 1);
+  p.owner = p.entries + (p.tensors > kTable ? sizeof(Entry) * (size_t)p.tensors : 0);
+  p.total = p.owner + (p.tensors > kTable ? sizeof(uint32_t) * (size_t)p.chunks : 0);
+  return true;
 }
 
 struct Range {
@@ -380,21 +424,21 @@ int overlap(const ganamd_tensor* l, int n) {
   return bad;
 }
 
-// Calls f(table) for the list's launches; tensors without elements take no place.
+// Calls f(table) for the pieces of a list that fit a launch; tensors without elements take no place.
 template <class F>
 int for_tables(const ganamd_tensor* l, int n, long chunk, F f) {
   Table t;
   t.n = 0;
   t.chunk = (int)chunk;
-  t.chunks = t.base = 0;
+  t.chunks = t.base = t.index = 0;
   for (int i = 0; i <= n; ++i) {
     if (i == n || t.n == kTable) {
       if (t.n) {
         f(t);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return GANAMD_ELAUNCH;
+        if (hipGetLastError() != hipSuccess) return GANAMD_ELAUNCH;
       }
       t.base += t.chunks;
+      t.index += t.n;
       t.n = 0;
       t.chunks = 0;
       if (i == n) break;
@@ -411,25 +455,47 @@ int for_tables(const ganamd_tensor* l, int n, long chunk, F f) {
   return GANAMD_OK;
 }
 
+// f(table) once for the whole list: of the arguments' kind, or of the workspace's, laid out first.
+template <class F>
+int for_list(const ganamd_tensor* l, int n, const Plan& p, char* ws, bool lay, hipStream_t st, F f) {
+  if (p.tensors <= kTable) return for_tables(l, n, p.chunk, f);
+  Entry* e = reinterpret_cast<Entry*>(ws + p.entries);
+  uint32_t* owner = reinterpret_cast<uint32_t*>(ws + p.owner);
+  if (lay) {
+    const int rc = for_tables(l, n, p.chunk, [&](const Table& t) {
+      hipLaunchKernelGGL(list_kernel, dim3(t.n), dim3(kNT), 0, st, t, e, owner);
+    });
+    if (rc != GANAMD_OK) return rc;
+  }
+  f(Listed{e, owner, p.tensors, (int)p.chunk, (uint32_t)p.chunks});
+  return ok(hipGetLastError());
+}
+
 template <int KIND>
-int norm_launches(const ganamd_tensor* l, int n, long chunk, double* part, hipStream_t st) {
-  return for_tables(l, n, chunk, [&](const Table& t) {
-    hipLaunchKernelGGL(norm_kernel<KIND>, dim3(t.chunks), dim3(kNT), 0, st, t, part);
+int norm_launches(const ganamd_tensor* l, int n, const Plan& p, char* ws, hipStream_t st) {
+  return for_list(l, n, p, ws, true, st, [&](const auto& t) {
+    hipLaunchKernelGGL((norm_kernel<KIND, std::decay_t<decltype(t)>>), dim3(t.chunks), dim3(kNT), 0, st, t,
+                       reinterpret_cast<double*>(ws));
   });
 }
 
 template <int KIND>
-int clip(const ganamd_tensor* l, int n, long chunk, long chunks, float max_norm, float* norm, double* part,
-         hipStream_t st) {
-  int rc = norm_launches<KIND>(l, n, chunk, part, st);
+int fold_launch(const Plan& p, float* norm, char* ws, hipStream_t st) {
+  double* part = reinterpret_cast<double*>(ws);
+  hipLaunchKernelGGL(norm_fold_kernel<KIND>, dim3(1), dim3(1024), 0, st, part, p.chunks, norm, part + p.chunks);
+  return ok(hipGetLastError());
+}
+
+template <int KIND>
+int clip(const ganamd_tensor* l, int n, const Plan& p, float max_norm, float* norm, char* ws, hipStream_t st) {
+  int rc = norm_launches<KIND>(l, n, p, ws, st);
+  const bool alone = p.chunks == 0 || p.chunks > kFoldMax;
+  if (rc == GANAMD_OK && alone) rc = fold_launch<KIND>(p, norm, ws, st);
   if (rc != GANAMD_OK) return rc;
-  const bool alone = chunks == 0 || chunks > kFoldMax;
-  double* total = part + chunks;
-  if (alone) hipLaunchKernelGGL(norm_fold_kernel<KIND>, dim3(1), dim3(1024), 0, st, part, chunks, norm, total);
-  if (hipGetLastError() != hipSuccess) return GANAMD_ELAUNCH;
-  return for_tables(l, n, chunk, [&](const Table& t) {
-    hipLaunchKernelGGL(scale_kernel<KIND>, dim3(t.chunks), dim3(kNT), 0, st, t, alone ? total : part,
-                       alone ? 0 : (int)chunks, max_norm, alone ? nullptr : norm);
+  const double* part = reinterpret_cast<const double*>(ws);
+  return for_list(l, n, p, ws, false, st, [&](const auto& t) {
+    hipLaunchKernelGGL((scale_kernel<KIND, std::decay_t<decltype(t)>>), dim3(t.chunks), dim3(kNT), 0, st, t,
+                       alone ? part + p.chunks : part, alone ? 0 : (int)p.chunks, max_norm, alone ? nullptr : norm);
   });
 }
 
@@ -438,42 +504,34 @@ int clip(const ganamd_tensor* l, int n, long chunk, long chunks, float max_norm,
 extern "C" {
 
 size_t ganamd_grad_norm_workspace(const ganamd_tensor* list, int n) {
-  long chunk;
-  const long c = plan(list, n, chunk);
-  return c < 0 ? 0 : sizeof(double) * ((size_t)c + 1);
+  Plan p;
+  return plan(list, n, p) ? p.total : 0;
 }
 
 int ganamd_grad_norm(const ganamd_tensor* list, int n, int kind, float* norm, void* workspace, size_t workspace_bytes,
                      hipStream_t st) {
-  long chunk;
-  const long chunks = plan(list, n, chunk);
-  if (chunks < 0 || !norm || !workspace || workspace_bytes < sizeof(double) * ((size_t)chunks + 1) ||
+  Plan p;
+  if (!plan(list, n, p) || !norm || !workspace || workspace_bytes < p.total ||
       (kind != GANAMD_NORM_L2 && kind != GANAMD_NORM_MAX))
     return GANAMD_EINVAL;
-  double* part = static_cast<double*>(workspace);
-  const int rc = kind == GANAMD_NORM_L2 ? norm_launches<0>(list, n, chunk, part, st) : norm_launches<1>(list, n, chunk, part, st);
+  char* ws = static_cast<char*>(workspace);
+  const int rc = kind == GANAMD_NORM_L2 ? norm_launches<0>(list, n, p, ws, st) : norm_launches<1>(list, n, p, ws, st);
   if (rc != GANAMD_OK) return rc;
-  if (kind == GANAMD_NORM_L2)
-    hipLaunchKernelGGL(norm_fold_kernel<0>, dim3(1), dim3(1024), 0, st, part, chunks, norm, (double*)nullptr);
-  else
-    hipLaunchKernelGGL(norm_fold_kernel<1>, dim3(1), dim3(1024), 0, st, part, chunks, norm, (double*)nullptr);
-  return ok(hipGetLastError());
+  return kind == GANAMD_NORM_L2 ? fold_launch<0>(p, norm, ws, st) : fold_launch<1>(p, norm, ws, st);
 }
 
 int ganamd_grad_clip(const ganamd_tensor* list, int n, int kind, float max_norm, float* norm, void* workspace,
                      size_t workspace_bytes, hipStream_t st) {
-  long chunk;
-  const long chunks = plan(list, n, chunk);
-  if (chunks < 0 || !norm || !workspace || workspace_bytes < sizeof(double) * ((size_t)chunks + 1) ||
+  Plan p;
+  if (!plan(list, n, p) || !norm || !workspace || workspace_bytes < p.total ||
       (kind != GANAMD_NORM_L2 && kind != GANAMD_NORM_MAX) || !(max_norm >= 0.f))
     return GANAMD_EINVAL;
   for (int i = 0; i < n; ++i)
     if ((list[i].n && !list[i].out) || (list[i].out_dtype != list[i].dtype && list[i].out_dtype != GANAMD_F32))
       return GANAMD_EINVAL;
   if (overlap(list, n) != 0) return GANAMD_EINVAL;
-  double* part = static_cast<double*>(workspace);
-  return kind == GANAMD_NORM_L2 ? clip<0>(list, n, chunk, chunks, max_norm, norm, part, st)
-                                : clip<1>(list, n, chunk, chunks, max_norm, norm, part, st);
+  char* ws = static_cast<char*>(workspace);
+  return kind == GANAMD_NORM_L2 ? clip<0>(list, n, p, max_norm, norm, ws, st) : clip<1>(list, n, p, max_norm, norm, ws, st);
 }
 
 size_t ganamd_adamw_clip_workspace(void) { return sizeof(double) * kStepBlocks; }
@@ -481,18 +539,17 @@ size_t ganamd_adamw_clip_workspace(void) { return sizeof(double) * kStepBlocks; 
 int ganamd_adamw_clip(float* p, const float* g, float* m, float* v, long n, int32_t* step, double lr, double beta1,
                       double beta2, double eps, double weight_decay, float max_norm, float* norm, void* workspace,
                       size_t workspace_bytes, hipStream_t st) {
-  if (!p || !g || !m || !v || !step || !norm || n <= 0 || !(max_norm >= 0.f) || !workspace ||
+  const long blocks = std::max<long>(1, (n / 4 + kNT * kStepVec - 1) / (kNT * kStepVec));
+  if (!p || !g || !m || !v || !step || !norm || n <= 0 || blocks >= (1L << 31) || !(max_norm >= 0.f) || !workspace ||
       workspace_bytes < ganamd_adamw_clip_workspace())
     return GANAMD_EINVAL;
   double* part = static_cast<double*>(workspace);
-  // whole vectors a thread and trip: 4 vectors of 4 elements
-  const long unit = 16L * kNT;
+  const long unit = 16L * kNT;                        // whole trips of norm_chunk
   const long per = std::max(unit, ((n + kStepBlocks - 1) / kStepBlocks + unit - 1) / unit * unit);
   const int parts = (int)((n + per - 1) / per);
   hipLaunchKernelGGL(flat_norm_kernel, dim3(parts), dim3(kNT), 0, st, g, n, per, part, step);
-  const long blocks = std::min<long>(2048, std::max<long>(1, (n / 4 + kNT - 1) / kNT));
-  hipLaunchKernelGGL(adamw_clip_kernel, dim3((unsigned)blocks), dim3(kNT), 0, st, p, g, m, v, n, part, parts, step, lr,
-                     beta1, beta2, eps, weight_decay, max_norm, norm);
+  hipLaunchKernelGGL(adamw_clip_kernel, dim3((unsigned)blocks), dim3(kNT), 0, st, p, g, m, v, n, part, parts, step,
+                     AdamArgs{lr, beta1, beta2, eps, weight_decay, max_norm}, norm);
   return ok(hipGetLastError());
 }
 
