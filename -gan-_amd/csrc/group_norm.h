@@ -828,58 +828,72 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
 #define GN_UD 2
 #define GN_UA 2
 #endif
-#ifndef GN_PF
-#define GN_PF 1
-#endif
 #ifndef GN_BLOCKS
 #define GN_BLOCKS 512
 #endif
 constexpr int kNT = 512;
 
-// The loop of both passes over a chunk: U positions at a time, the next ones loaded before the
-// present ones are used; `first` runs between the first loads and their use.
+// The loop of both passes over a chunk: U positions a trip, the next ones loaded before the present
+// ones are used; `first` runs between the first loads and their use.  use(at, skip, x, gy, v) gets
+// skip == 0 where nothing is moved back (rows: a thread's own skip0); only the last trip looks at
+// the chunk's end, and at the end of a plane.
 template <int MODE, bool ROWS, class T, int V, int U, class First, class Use>
 __device__ __forceinline__ void stream(const Args& a, const Map<ROWS, V>& m, int lo, int hi, First first, Use use) {
   const T* px = static_cast<const T*>(a.x);
   const T* pg = static_cast<const T*>(a.gy);
   const T* pv = static_cast<const T*>(a.v);
   Vec<T, V> x[U], gy[MODE >= BWD ? U : 1], v[MODE == DBL ? U : 1];
-  long at[U];
-  int skip[U];
-  const int step = U * a.P;
-  auto fetch = [&](int i0) {
+  const int whole = ROWS ? hi : min(hi, (int)(a.L / V));       // positions before it are whole vectors
+  const long hop = (long)a.P * m.step;
+  int i0 = lo + m.p;
+  auto fetch = [&](int i, bool full) {
+    const long at = m.base + i * m.step;
+    if (full) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * a.P;
-      skip[u] = V;
-      if (i < hi) {
-        at[u] = m.at(i, skip[u]);
-        x[u] = load<T, V>(px + at[u]);
-        if constexpr (MODE >= BWD) gy[u] = load<T, V>(pg + at[u]);
-        if constexpr (MODE == DBL) v[u] = load<T, V>(pv + at[u]);
+      for (int u = 0; u < U; ++u) {
+        x[u] = load<T, V>(px + at + u * hop);
+        if constexpr (MODE >= BWD) gy[u] = load<T, V>(pg + at + u * hop);
+        if constexpr (MODE == DBL) v[u] = load<T, V>(pv + at + u * hop);
       }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * a.P < hi) {
+          int skip;
+          const long q = m.at(i + u * a.P, skip);
+          x[u] = load<T, V>(px + q);
+          if constexpr (MODE >= BWD) gy[u] = load<T, V>(pg + q);
+          if constexpr (MODE == DBL) v[u] = load<T, V>(pv + q);
+        }
     }
   };
-  if (m.active) fetch(lo + m.p);
+  bool full = i0 + (U - 1) * a.P < whole;
+  if (m.active) fetch(i0, full);
   first();
   if (!m.active) return;
-  for (int i0 = lo + m.p; i0 < hi; i0 += step) {
+  while (full) {
     Vec<T, V> cx[U], cg[MODE >= BWD ? U : 1], cv[MODE == DBL ? U : 1];
-    long ca[U];
-    int cs[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       cx[u] = x[u];
       if constexpr (MODE >= BWD) cg[u] = gy[u];
       if constexpr (MODE == DBL) cv[u] = v[u];
-      ca[u] = at[u];
-      cs[u] = skip[u];
     }
-    if (GN_PF && i0 + step < hi) fetch(i0 + step);
+    const long at = m.base + i0 * m.step;
+    i0 += U * a.P;
+    full = i0 + (U - 1) * a.P < whole;
+    fetch(i0, full);
 #pragma unroll
-    for (int u = 0; u < U; ++u) use(ca[u], cs[u], cx[u], cg[MODE >= BWD ? u : 0], cv[MODE == DBL ? u : 0]);
-    if (!GN_PF && i0 + step < hi) fetch(i0 + step);
+    for (int u = 0; u < U; ++u)
+      use(at + u * hop, ROWS ? m.skip0 : 0, cx[u], cg[MODE >= BWD ? u : 0], cv[MODE == DBL ? u : 0]);
   }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (i0 + u * a.P < hi) {
+      int skip;
+      const long at = m.at(i0 + u * a.P, skip);
+      use(at, skip, x[u], gy[MODE >= BWD ? u : 0], v[MODE == DBL ? u : 0]);
+    }
 }
 
 // blockIdx.x = (sample, tile, chunk), chunk fastest
@@ -906,9 +920,11 @@ __global__ __launch_bounds__(kNT) void sums_kernel(Args a) {
   stream<MODE, ROWS, T, V, U>(
       a, m, s * a.per, hi, [&] { load_chan<MODE, ACT, ROWS, V, NC>(a, m, b, c0, tab, ch); },
       [&](long, int skip, Vec<T, V>& x, Vec<T, V>& gy, Vec<T, V>& v) {
-        if (MODE == FWD || skip == V) x.zero_front(skip);
-        if constexpr (MODE >= BWD) gy.zero_front(skip);
-        if constexpr (MODE == DBL) v.zero_front(skip);
+        if constexpr (!ROWS) {                 // (rows: the fold leaves a moved-back front out)
+          if (MODE == FWD) x.zero_front(skip);
+          if constexpr (MODE >= BWD) gy.zero_front(skip);
+          if constexpr (MODE == DBL) v.zero_front(skip);
+        }
         accumulate<MODE, ACT, ROWS, T, V, NC>(acc, ch, x, gy, v);
       });
   fold<ROWS, V, K, NC>(a, m, acc, sh, chan, c0);
@@ -982,7 +998,7 @@ __global__ __launch_bounds__(kNT) void apply_kernel(Args a) {
                                          reinterpret_cast<float*>(lds), ln);
       },
       [&](long at, int skip, Vec<T, V>& x, Vec<T, V>& gy, Vec<T, V>& v) {
-        if (skip < V) write<MODE, ACT, ROWS, T, V, NC>(a, ln, at, skip, x, gy, v);
+        write<MODE, ACT, ROWS, T, V, NC>(a, ln, at, skip, x, gy, v);
       });
 }
 
