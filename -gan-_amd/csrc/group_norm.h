@@ -38,7 +38,7 @@ namespace gn {
 enum { FWD = 0, BWD = 1, DBL = 2 };
 enum { SILU = 0, KINK = 1, SLOPE = 2 };   // SLOPE: a kinked activation whose slope has a gradient
 
-// One operator call on one batch slice, as the kernels see it.
+// One operator call as the kernels see it.
 struct Args {
   const void *x, *gy, *v;                       // data, in T
   void *o1, *o2;                                // y | gx | g_gy, g_x
@@ -49,8 +49,7 @@ struct Args {
   float* par;                                   // [3][B][C]: each sample's terms of gw, gb, gslope
   float cslope;                                 // constant slope where slope is null
   float eps;
-  long L, B;                                    // positions, samples of the whole tensor (strides)
-  int b0;                                       // first sample of this slice
+  long L, B;                                    // positions, samples
   int C, G, Cg, pdt;
   int TX, P;                                    // threads across the channels (rows) / planes per block; positions in flight
   int CT, nct;                                  // channels per tile, tiles
@@ -758,7 +757,7 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
   constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K;
   extern __shared__ __align__(16) char lds[];
   const int tile = blockIdx.x % a.nct;
-  const long b = a.b0 + blockIdx.x / a.nct;
+  const long b = blockIdx.x / a.nct;
   const Map<ROWS, V> m(a, b, tile);
   const int gt = a.CT / a.Cg;                       // groups of a tile (the last may hold fewer)
   double* gco = reinterpret_cast<double*>(lds);     // [gt][8] (FWD: mean, r)
@@ -823,14 +822,6 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
 }
 
 // ------------------------------------------------------------------ the split form
-#ifndef GN_US
-#define GN_US 4
-#define GN_UD 2
-#define GN_UA 2
-#endif
-#ifndef GN_BLOCKS
-#define GN_BLOCKS 512
-#endif
 constexpr int kNT = 512;
 
 // The loop of both passes over a chunk: U positions a trip, the next ones loaded before the present
@@ -900,11 +891,11 @@ __device__ __forceinline__ void stream(const Args& a, const Map<ROWS, V>& m, int
 template <int MODE, int ACT, bool ROWS, class T, int V>
 __global__ __launch_bounds__(kNT) void sums_kernel(Args a) {
   typedef typename AccT<MODE>::type A;
-  constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K, U = MODE == DBL ? GN_UD : GN_US;
+  constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K, U = 2;
   extern __shared__ __align__(16) char lds[];
   const int s = blockIdx.x % a.S, tile = blockIdx.x / a.S % a.nct;
   const int bi = blockIdx.x / a.S / a.nct;
-  const long b = a.b0 + bi;
+  const long b = bi;
   const Map<ROWS, V> m(a, b, tile);
   float* tab = reinterpret_cast<float*>(lds);
   A* chan = reinterpret_cast<A*>(lds);
@@ -954,7 +945,7 @@ __global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) 
   typedef typename AccT<MODE>::type A;
   constexpr int K = Sums<MODE, ACT>::K;
   const int nb = (a.G + gpb - 1) / gpb, g0 = blockIdx.x % nb * gpb, bi = blockIdx.x / nb;
-  const long b = a.b0 + bi;
+  const long b = bi;
   const int ng = min(gpb, a.G - g0), nc = ng * a.Cg, pairs = K * nc, ns = (a.S + sstep - 1) / sstep;
   A* part = reinterpret_cast<A*>(a.part) + (long)bi * a.S * K * a.C + g0 * a.Cg;
   if (ns > 1) {
@@ -982,10 +973,10 @@ __global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) 
 
 template <int MODE, int ACT, bool ROWS, class T, int V>
 __global__ __launch_bounds__(kNT) void apply_kernel(Args a) {
-  constexpr int NC = ROWS ? V : 1, U = GN_UA;
+  constexpr int NC = ROWS ? V : 1, U = 2;
   extern __shared__ __align__(16) char lds[];
   const int s = blockIdx.x % a.S, tile = blockIdx.x / a.S % a.nct;
-  const long b = a.b0 + blockIdx.x / a.S / a.nct;
+  const long b = blockIdx.x / a.S / a.nct;
   const Map<ROWS, V> m(a, b, tile);
   const int c0 = tile * a.CT;
   const int hi = (int)min((long)m.npos, (long)(s + 1) * a.per);
@@ -1014,66 +1005,72 @@ struct Plan {
   bool rows, resident;
   int V, rmax, nt;
   size_t lds, apply_lds;
+  int apply_S, apply_per; // the elementwise pass's own chunks
   int gpb, sstep;         // groups a folding block takes; chunks are folded by 32 before (or 1)
-  int slice;              // samples per slice
 };
 
 template <int MODE, int ACT, bool ROWS, class T, int V, int RMAX>
-int launch_resident(const Plan& p, const Args& a, long nb, hipStream_t st) {
+int launch_resident(const Plan& p, const Args& a, hipStream_t st) {
   constexpr int NTMAX = resident_threads(MODE, ROWS);
-  hipLaunchKernelGGL((resident_kernel<MODE, ACT, ROWS, T, V, RMAX, NTMAX>), dim3((unsigned)(nb * a.nct)), dim3(p.nt),
+  hipLaunchKernelGGL((resident_kernel<MODE, ACT, ROWS, T, V, RMAX, NTMAX>), dim3((unsigned)(a.B * a.nct)), dim3(p.nt),
                      p.lds, st, a);
   return hipGetLastError() == hipSuccess ? GANAMD_OK : GANAMD_ELAUNCH;
 }
 
 template <int MODE, int ACT, bool ROWS, class T, int V>
-int launch_v(const Plan& p, const Args& a, long nb, hipStream_t st) {
+int launch_v(const Plan& p, const Args& a, hipStream_t st) {
   if (p.resident) {
     constexpr int MOST = resident_vectors(MODE);
-    if (p.rmax <= 2) return launch_resident<MODE, ACT, ROWS, T, V, 2>(p, a, nb, st);
-    if (p.rmax <= MOST / 2) return launch_resident<MODE, ACT, ROWS, T, V, MOST / 2>(p, a, nb, st);
-    return launch_resident<MODE, ACT, ROWS, T, V, MOST>(p, a, nb, st);
+    if (p.rmax <= 2) return launch_resident<MODE, ACT, ROWS, T, V, 2>(p, a, st);
+    if (p.rmax <= MOST / 2) return launch_resident<MODE, ACT, ROWS, T, V, MOST / 2>(p, a, st);
+    return launch_resident<MODE, ACT, ROWS, T, V, MOST>(p, a, st);
   }
-  const dim3 grid((unsigned)(nb * a.nct * a.S));
+  const dim3 grid((unsigned)(a.B * a.nct * a.S));
   hipLaunchKernelGGL((sums_kernel<MODE, ACT, ROWS, T, V>), grid, dim3(p.nt), p.lds, st, a);
   if (p.sstep > 1) {
     typedef typename AccT<MODE>::type A;
     const int n = Sums<MODE, ACT>::K * a.C;
-    hipLaunchKernelGGL(chunk_kernel<A>, dim3((n + 255) / 256, (a.S + kFold - 1) / kFold, (unsigned)nb), dim3(256), 0,
+    hipLaunchKernelGGL(chunk_kernel<A>, dim3((n + 255) / 256, (a.S + kFold - 1) / kFold, (unsigned)a.B), dim3(256), 0,
                        st, reinterpret_cast<A*>(a.part), a.S, n);
   }
-  hipLaunchKernelGGL((group_kernel<MODE, ACT>), dim3((unsigned)(nb * ((a.G + p.gpb - 1) / p.gpb))), dim3(256),
+  hipLaunchKernelGGL((group_kernel<MODE, ACT>), dim3((unsigned)(a.B * ((a.G + p.gpb - 1) / p.gpb))), dim3(256),
                      MODE == FWD ? 64 * (size_t)p.gpb : 0, st, a, p.gpb, p.sstep);
-  if (MODE != BWD || a.o1)
-    hipLaunchKernelGGL((apply_kernel<MODE, ACT, ROWS, T, V>), grid, dim3(p.nt), p.apply_lds, st, a);
+  if (MODE != BWD || a.o1) {
+    Args b = a;
+    b.S = p.apply_S;
+    b.per = p.apply_per;
+    hipLaunchKernelGGL((apply_kernel<MODE, ACT, ROWS, T, V>), dim3((unsigned)(a.B * a.nct * b.S)), dim3(p.nt), p.apply_lds,
+                       st, b);
+  }
   return hipGetLastError() == hipSuccess ? GANAMD_OK : GANAMD_ELAUNCH;
 }
 
-// vector width of an element type: 16 bytes; 4 elements where a thread carries the sums and
-// coefficients of each of its channels (rows, backward), 1 where rows / planes are shorter
-constexpr int vec_width(int mode, bool rows, int size) { return rows && mode != FWD ? 4 : 16 / size; }
+// Vector width of an element type: 16 bytes; in the double backward of rows, where a thread carries
+// ten sums and a dozen coefficients of each of its channels, 4 elements; 1 where rows or planes are
+// shorter than that.
+constexpr int vec_width(int mode, bool rows, int size) { return rows && mode == DBL ? 4 : 16 / size; }
 
 template <int MODE, int ACT, class T>
-int launch_t(const Plan& p, const Args& a, long nb, hipStream_t st) {
+int launch_t(const Plan& p, const Args& a, hipStream_t st) {
   constexpr int VR = vec_width(MODE, true, sizeof(T)), VP = vec_width(MODE, false, sizeof(T));
-  if (p.rows) return p.V == 1 ? launch_v<MODE, ACT, true, T, 1>(p, a, nb, st) : launch_v<MODE, ACT, true, T, VR>(p, a, nb, st);
-  return p.V == 1 ? launch_v<MODE, ACT, false, T, 1>(p, a, nb, st) : launch_v<MODE, ACT, false, T, VP>(p, a, nb, st);
+  if (p.rows) return p.V == 1 ? launch_v<MODE, ACT, true, T, 1>(p, a, st) : launch_v<MODE, ACT, true, T, VR>(p, a, st);
+  return p.V == 1 ? launch_v<MODE, ACT, false, T, 1>(p, a, st) : launch_v<MODE, ACT, false, T, VP>(p, a, st);
 }
 
 template <class T>
-int launch(const Plan& p, const Args& a, long nb, hipStream_t st) {
+int launch(const Plan& p, const Args& a, hipStream_t st) {
   if (p.mode == FWD)
-    return p.act == SILU ? launch_t<FWD, SILU, T>(p, a, nb, st) : launch_t<FWD, KINK, T>(p, a, nb, st);
+    return p.act == SILU ? launch_t<FWD, SILU, T>(p, a, st) : launch_t<FWD, KINK, T>(p, a, st);
   if (p.mode == BWD)
-    return p.act == SILU ? launch_t<BWD, SILU, T>(p, a, nb, st)
-         : p.act == KINK ? launch_t<BWD, KINK, T>(p, a, nb, st) : launch_t<BWD, SLOPE, T>(p, a, nb, st);
-  return p.act == SILU ? launch_t<DBL, SILU, T>(p, a, nb, st)
-       : p.act == KINK ? launch_t<DBL, KINK, T>(p, a, nb, st) : launch_t<DBL, SLOPE, T>(p, a, nb, st);
+    return p.act == SILU ? launch_t<BWD, SILU, T>(p, a, st)
+         : p.act == KINK ? launch_t<BWD, KINK, T>(p, a, st) : launch_t<BWD, SLOPE, T>(p, a, st);
+  return p.act == SILU ? launch_t<DBL, SILU, T>(p, a, st)
+       : p.act == KINK ? launch_t<DBL, KINK, T>(p, a, st) : launch_t<DBL, SLOPE, T>(p, a, st);
 }
 
 // one translation unit per element type (compiled in parallel)
-int launch_f32(const Plan& p, const Args& a, long nb, hipStream_t st);
-int launch_bf16(const Plan& p, const Args& a, long nb, hipStream_t st);
-int launch_f16(const Plan& p, const Args& a, long nb, hipStream_t st);
+int launch_f32(const Plan& p, const Args& a, hipStream_t st);
+int launch_bf16(const Plan& p, const Args& a, hipStream_t st);
+int launch_f16(const Plan& p, const Args& a, hipStream_t st);
 
 }  // namespace gn

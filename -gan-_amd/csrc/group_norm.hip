@@ -55,7 +55,6 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   a.L = L; a.B = B; a.C = C; a.G = G; a.Cg = Cg; a.eps = d->eps; a.pdt = d->param_dtype;
   a.cslope = d->act == GANAMD_NORM_LEAKY ? d->slope : 1.f;
   p.resident = false;
-  p.slice = (int)B;
   const long nv = up_to(L, p.V);
   if (p.rows) {
     // a tile of whole groups, at least a cache line wide
@@ -84,8 +83,8 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     }
   }
   if (p.resident) {
-    a.S = 1;
-    a.per = 0;
+    a.S = p.apply_S = 1;
+    a.per = p.apply_per = 0;
     const size_t sh = p.rows ? (size_t)gn::fold_round(K, p.V, p.nt, asz) * p.V * p.nt : (size_t)K * 16;
     p.lds = (size_t)(a.CT / Cg) * 64 + std::max(asz * ((size_t)K * a.CT + sh), 4 * (size_t)tabs * a.CT);
     if (p.lds > 64 * 1024) p.resident = false;
@@ -109,31 +108,31 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
       p.nt = (int)up_to((long)a.TX * a.P, 64) * 64;
       npos = nv;
     }
-    // four blocks of eight waves a CU, but four vectors a thread at least, and at most 128 values of
-    // a channel in one thread's fp32 sums
-#ifdef GN_SLICE
-    {
-      const long per_sample = (mode == gn::FWD ? 2 : mode == gn::BWD ? 3 : 5) * L * C * esz;
-      const long n = std::max<long>(1, (GN_SLICE * 1048576L) / per_sample);
-      if (n < B) p.slice = (int)up_to(B, up_to(B, n));
-    }
-#endif
-    const long nb = p.slice;
-    long S = std::max<long>(1, std::min(up_to(GN_BLOCKS, nb * a.nct), up_to(npos, 4L * a.P)));
+    // The sums: two blocks of eight waves a CU, but four vectors a thread at least (more blocks are
+    // more folds: 64 maps of 64x64x96 in bf16 took 37 us with 512 blocks, 42 with 1024, 48 with
+    // 2048), and at most 128 values of a channel in one thread's fp32 sums.
+    long S = std::max<long>(1, std::min(up_to(512, B * a.nct), up_to(npos, 4L * a.P)));
     S = std::max(S, up_to(npos, (p.rows ? 128L : 128L / p.V) * a.P));
     a.per = (int)(up_to(up_to(npos, S), a.P) * a.P);
     a.S = (int)up_to(npos, a.per);
+    // The elementwise pass: as many, while its tensors fit the 256 MB of the last-level cache; beyond,
+    // pieces in launch order, which keep what is in flight together in memory (backward of 256 such
+    // maps: 203 us with 8192 blocks, 229 with 512; of 64 maps of 64x64x64 in fp32 121 against 116).
+    const long data = (mode == gn::FWD ? 2 : mode == gn::BWD ? 3 : 5) * B * L * C * esz;
+    const long SA = std::max<long>(1, std::min(up_to(data > (256L << 20) ? 8192 : 512, B * a.nct), up_to(npos, 4L * a.P)));
+    p.apply_per = (int)(up_to(up_to(npos, SA), a.P) * a.P);
+    p.apply_S = (int)up_to(npos, p.apply_per);
     const size_t sh = p.rows ? (size_t)gn::fold_round(K, p.V, p.nt, asz) * p.V * p.nt : (size_t)K * 16;
     p.lds = std::max(asz * ((size_t)K * a.CT + sh), 4 * (size_t)tabs * a.CT);
     p.apply_lds = 4 * (size_t)tabs * a.CT;
   }
   p.gpb = (int)std::max<long>(1, std::min<long>(G, 256 / ((long)K * Cg)));
   p.sstep = a.S > 2 * gn::kFold ? gn::kFold : 1;
-  if (B * a.nct * a.S >= (1L << 31) || B * G >= (1L << 31) || p.lds > 64 * 1024) return false;
+  if (B * a.nct * std::max(a.S, p.apply_S) >= (1L << 31) || B * G >= (1L << 31) || p.lds > 64 * 1024) return false;
   // workspace
   size_t at = 0;
   auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
-  f.part = p.resident ? 0 : take(asz * (size_t)K * C * a.S * p.slice);
+  f.part = p.resident ? 0 : take(asz * (size_t)K * C * a.S * B);
   f.coef = p.resident || mode == gn::FWD ? 0 : take(64 * (size_t)B * G);
   f.par = mode == gn::FWD ? 0 : take(4 * 3 * (size_t)B * C);
   f.fold = mode == gn::FWD || B <= kFoldB ? 0 : take(4 * 3 * (size_t)up_to(B, kFoldB) * C);
@@ -201,14 +200,8 @@ int fold_params(const Full& f, char* ws, int K, void* gw, void* gb, void* gs, in
 int run(const ganamd_norm_desc* d, const Full& f, Args a, char* ws, hipStream_t st) {
   a.part = reinterpret_cast<float*>(ws + f.part);
   a.coef = reinterpret_cast<double*>(ws + f.coef);
-  for (long b0 = 0; b0 < f.a.B; b0 += f.p.slice) {
-    a.b0 = (int)b0;
-    const long nb = std::min<long>(f.p.slice, f.a.B - b0);
-    const int rc = d->dtype == GANAMD_F32 ? gn::launch_f32(f.p, a, nb, st)
-                 : d->dtype == GANAMD_BF16 ? gn::launch_bf16(f.p, a, nb, st) : gn::launch_f16(f.p, a, nb, st);
-    if (rc != GANAMD_OK) return rc;
-  }
-  return GANAMD_OK;
+  return d->dtype == GANAMD_F32 ? gn::launch_f32(f.p, a, st)
+       : d->dtype == GANAMD_BF16 ? gn::launch_bf16(f.p, a, st) : gn::launch_f16(f.p, a, st);
 }
 
 }  // namespace
@@ -225,8 +218,9 @@ int ganamd_group_norm_workspace(const ganamd_norm_desc* d, int op, size_t* bytes
 int ganamd_group_norm_plan_info(const ganamd_norm_desc* d, int op, int* info) {
   Full f;
   if (!info || op < gn::FWD || op > gn::DBL || !make_plan(d, op, f)) return GANAMD_EINVAL;
-  const int v[10] = {f.p.resident, f.p.V, f.p.nt, f.a.TX, f.a.P, f.a.CT, f.a.nct, f.a.S, f.a.per, f.p.slice};
-  for (int i = 0; i < 10; ++i) info[i] = v[i];
+  const int v[11] = {f.p.resident, f.p.V,  f.p.nt, f.a.TX,      f.a.P,        f.a.CT,
+                     f.a.nct,      f.a.S, f.a.per, f.p.apply_S, f.p.apply_per};
+  for (int i = 0; i < 11; ++i) info[i] = v[i];
   return GANAMD_OK;
 }
 

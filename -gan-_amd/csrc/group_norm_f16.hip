@@ -2,5 +2,5 @@
 #include "group_norm.h"
 
 namespace gn {
-int launch_f16(const Plan& p, const Args& a, long nb, hipStream_t st) { return launch<f16>(p, a, nb, st); }
+int launch_f16(const Plan& p, const Args& a, hipStream_t st) { return launch<f16>(p, a, st); }
 }  // namespace gn

@@ -299,9 +299,9 @@ typedef struct ganamd_norm_desc {
 
 /* Workspace bytes of the forward (op 0), backward (1) and double backward (2); may be 0. */
 int ganamd_group_norm_workspace(const ganamd_norm_desc* d, int op, size_t* bytes);
-/* The launch a call takes: info[10] = {one-launch form, vector width, threads, threads across /
- * planes per block, positions in flight, channels per tile, tiles, chunks, positions per chunk,
- * samples per slice} (introspection for tests). */
+/* The launch a call takes: info[11] = {one-launch form, vector width, threads, threads across /
+ * planes per block, positions in flight, channels per tile, tiles, chunks, positions per chunk of the
+ * sums, and of the elementwise pass} (introspection for tests). */
 int ganamd_group_norm_plan_info(const ganamd_norm_desc* d, int op, int* info);
 int ganamd_group_norm_fwd(const ganamd_norm_desc* d, const void* x, const void* w, const void* b, const void* slope,
                           void* y, double* stats, void* workspace, size_t workspace_bytes, hipStream_t stream);

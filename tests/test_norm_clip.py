@@ -90,10 +90,10 @@ def plan(shape, G, dtype, act, layout, op):
     B, C = (shape[0], shape[-1]) if layout == "nhwc" else (shape[1], shape[0])
     d = _lib.NormDesc(math.prod(shape) // (B * C), B, C, G, ("nhwc", "cnhw").index(layout),
                       (torch.float32, torch.bfloat16, torch.float16).index(dtype), 0, ACTS.index(act), 0.2, 1e-5)
-    info, n = (ctypes.c_int * 10)(), _lib.c_size_t(0)
+    info, n = (ctypes.c_int * 11)(), _lib.c_size_t(0)
     assert _lib.LIB.ganamd_group_norm_plan_info(d, op, info) == 0
     assert _lib.LIB.ganamd_group_norm_workspace(d, op, n) == 0
-    keys = ("resident", "V", "nt", "TX", "P", "CT", "nct", "S", "per", "slice")
+    keys = ("resident", "V", "nt", "TX", "P", "CT", "nct", "S", "per", "SA", "perA")
     return dict(zip(keys, info)), n.value
 
 
@@ -123,12 +123,12 @@ def test_plan_owns_every_element_once(shape, G, layout, dtype):
             npos = L if rows else -(-L // V)
             if p["resident"]:
                 assert CT % (C // G) == 0
-                spans = [(0, npos)]
                 assert -(-npos // P) <= (8 if op == 2 else 16)
             else:
-                spans = [(s * p["per"], min(npos, (s + 1) * p["per"])) for s in range(p["S"])]
-                assert spans[0][0] == 0 and spans[-1][1] == npos
-                assert all(a < b for a, b in spans) and all(x[1] == y[0] for x, y in zip(spans, spans[1:]))
+                for S, per in ((p["S"], p["per"]), (p["SA"], p["perA"])):
+                    spans = [(s * per, min(npos, (s + 1) * per)) for s in range(S)]
+                    assert spans[0][0] == 0 and spans[-1][1] == npos
+                    assert all(a < b for a, b in spans) and all(x[1] == y[0] for x, y in zip(spans, spans[1:]))
             if not rows:
                 assert P & (P - 1) == 0
             assert (p["nct"] - 1) * CT < C <= p["nct"] * CT
