@@ -994,10 +994,10 @@ __global__ __launch_bounds__(kNT) void apply_kernel(Args a) {
 }
 
 // ------------------------------------------------------------------ launches
-// Threads of a resident block and the vectors of each input that a thread can hold: what fits
-// 256 registers a thread (512 threads) or 128 (1024; one input).
-constexpr int resident_threads(int mode, bool rows) { return rows || mode != FWD ? 512 : 1024; }
-constexpr int resident_vectors(int mode) { return mode == DBL ? 8 : 16; }
+// Threads of a resident block and the vectors of each input that a thread can hold: what fits 128
+// registers a thread (1024 threads) or 256 (512).
+constexpr int resident_threads(int mode, bool rows) { return rows || mode == DBL ? 512 : 1024; }
+constexpr int resident_vectors(int mode, bool rows) { return mode == DBL || (mode == BWD && !rows) ? 8 : 16; }
 
 // How one call runs (group_norm.hip makes it from sizes and type alone).
 struct Plan {
@@ -1020,10 +1020,12 @@ int launch_resident(const Plan& p, const Args& a, hipStream_t st) {
 template <int MODE, int ACT, bool ROWS, class T, int V>
 int launch_v(const Plan& p, const Args& a, hipStream_t st) {
   if (p.resident) {
-    constexpr int MOST = resident_vectors(MODE);
+    constexpr int MOST = resident_vectors(MODE, ROWS);
     if (p.rmax <= 2) return launch_resident<MODE, ACT, ROWS, T, V, 2>(p, a, st);
-    if (p.rmax <= MOST / 2) return launch_resident<MODE, ACT, ROWS, T, V, MOST / 2>(p, a, st);
-    return launch_resident<MODE, ACT, ROWS, T, V, MOST>(p, a, st);
+    if (p.rmax <= 4) return launch_resident<MODE, ACT, ROWS, T, V, 4>(p, a, st);
+    if (p.rmax <= 8) return launch_resident<MODE, ACT, ROWS, T, V, 8>(p, a, st);
+    if constexpr (MOST > 8) return launch_resident<MODE, ACT, ROWS, T, V, MOST>(p, a, st);
+    return GANAMD_EINVAL;
   }
   const dim3 grid((unsigned)(a.B * a.nct * a.S));
   hipLaunchKernelGGL((sums_kernel<MODE, ACT, ROWS, T, V>), grid, dim3(p.nt), p.lds, st, a);

@@ -123,7 +123,7 @@ def test_plan_owns_every_element_once(shape, G, layout, dtype):
             npos = L if rows else -(-L // V)
             if p["resident"]:
                 assert CT % (C // G) == 0
-                assert -(-npos // P) <= (8 if op == 2 else 16)
+                assert -(-npos // P) <= (8 if op == 2 or (op == 1 and not rows) else 16)
             else:
                 for S, per in ((p["S"], p["per"]), (p["SA"], p["perA"])):
                     spans = [(s * per, min(npos, (s + 1) * per)) for s in range(S)]
