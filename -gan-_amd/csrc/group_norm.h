@@ -679,7 +679,7 @@ __device__ __forceinline__ void load_lin(const Args& a, const Map<ROWS, V>& m, l
 // terms of the parameter gradients to par.
 template <int MODE, int ACT, class A>
 __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int ng, const A* chan, long stride,
-                                              double* gco) {
+                                              double* gco, bool tell) {
   int W = 1;
   while (W < a.Cg && W < 64) W *= 2;
   const int lane = threadIdx.x & (W - 1), g0 = c0 / a.Cg;
@@ -702,8 +702,10 @@ __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int
       if (lane == 0) {
         co[0] = mean;
         co[1] = r;
-        st[0] = mean;
-        st[1] = r;
+        if (tell) {
+          st[0] = mean;
+          st[1] = r;
+        }
       }
     } else {
       const Group q = group_of(st[0], st[1]);
@@ -712,7 +714,7 @@ __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int
       for (int c = lane; c < a.Cg; c += W) {
         double terms[3];
         sweep1<MODE, ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * stride + cg + c]; }, m1, terms);
-        if (MODE == BWD && a.par)
+        if (MODE == BWD && tell && a.par)
 #pragma unroll
           for (int k = 0; k < Sums<BWD, ACT>::K; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
       }
@@ -728,7 +730,7 @@ __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int
         for (int c = lane; c < a.Cg; c += W) {
           double terms[3];
           sweep2<ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * stride + cg + c]; }, m1, m2, terms);
-          if (a.par)
+          if (tell && a.par)
 #pragma unroll
             for (int k = 0; k < 3; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
         }
@@ -802,7 +804,7 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
     if constexpr (MODE == DBL) v[k].pin();
   }
   fold<ROWS, V, K, NC>(a, m, acc, sh, chan, c0);
-  finish_groups<MODE, ACT>(a, b, c0, ng, chan, (long)a.CT, gco);
+  finish_groups<MODE, ACT>(a, b, c0, ng, chan, (long)a.CT, gco, true);
   __syncthreads();
   Lin<MODE, ACT> ln[NC];
   if (MODE == FWD)
@@ -968,12 +970,16 @@ __global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) 
   }
   // (FWD writes the statistics; the coefficients have their own place)
   extern __shared__ __align__(16) double gco[];
-  finish_groups<MODE, ACT>(a, b, g0 * a.Cg, ng, part, (long)a.C, MODE == FWD ? gco : a.coef + 8 * (b * a.G + g0));
+  finish_groups<MODE, ACT>(a, b, g0 * a.Cg, ng, part, (long)a.C, MODE == FWD ? gco : a.coef + 8 * (b * a.G + g0),
+                           true);
 }
 
-template <int MODE, int ACT, bool ROWS, class T, int V>
-__global__ __launch_bounds__(kNT) void apply_kernel(Args a) {
-  constexpr int NC = ROWS ? V : 1, U = 2;
+// FOLD: each block folds its sample's chunks and finishes the groups itself (rows, one tile of all
+// channels; a.part holds fold_S chunks), one launch less; else a group_kernel went before.
+template <int MODE, int ACT, bool ROWS, class T, int V, bool FOLD>
+__global__ __launch_bounds__(kNT) void apply_kernel(Args a, int fold_S) {
+  typedef typename AccT<MODE>::type A;
+  constexpr int NC = ROWS ? V : 1, K = Sums<MODE, ACT>::K, U = 2;
   extern __shared__ __align__(16) char lds[];
   const int s = blockIdx.x % a.S, tile = blockIdx.x / a.S % a.nct;
   const long b = blockIdx.x / a.S / a.nct;
@@ -985,8 +991,25 @@ __global__ __launch_bounds__(kNT) void apply_kernel(Args a) {
   stream<MODE, ROWS, T, V, U>(
       a, m, s * a.per, hi,
       [&] {
-        load_lin<MODE, ACT, ROWS, V, NC>(a, m, b, c0, a.stats + 2 * g0, 2, a.coef + 8 * g0,
-                                         reinterpret_cast<float*>(lds), ln);
+        if constexpr (FOLD) {
+          double* gco = reinterpret_cast<double*>(lds);
+          A* chan = reinterpret_cast<A*>(gco + 8L * a.G);            // [K][C]; then the coefficients
+          const A* part = reinterpret_cast<const A*>(a.part) + b * fold_S * K * a.C;
+          for (int i = threadIdx.x; i < K * a.C; i += blockDim.x) {
+            double t = 0;
+#pragma unroll 4
+            for (int k = 0; k < fold_S; ++k) t += (double)part[(long)k * K * a.C + i];
+            chan[i] = (A)t;
+          }
+          __syncthreads();
+          finish_groups<MODE, ACT>(a, b, 0, a.G, chan, (long)a.C, gco, s == 0);
+          __syncthreads();
+          load_lin<MODE, ACT, ROWS, V, NC>(a, m, b, 0, MODE == FWD ? gco : a.stats + 2 * g0, MODE == FWD ? 8 : 2, gco,
+                                           reinterpret_cast<float*>(chan), ln);
+        } else {
+          load_lin<MODE, ACT, ROWS, V, NC>(a, m, b, c0, a.stats + 2 * g0, 2, a.coef + 8 * g0,
+                                           reinterpret_cast<float*>(lds), ln);
+        }
       },
       [&](long at, int skip, Vec<T, V>& x, Vec<T, V>& gy, Vec<T, V>& v) {
         write<MODE, ACT, ROWS, T, V, NC>(a, ln, at, skip, x, gy, v);
@@ -1006,6 +1029,7 @@ struct Plan {
   int V, rmax, nt;
   size_t lds, apply_lds;
   int apply_S, apply_per; // the elementwise pass's own chunks
+  bool fold_apply;        // its blocks fold the sums' chunks themselves
   int gpb, sstep;         // groups a folding block takes; chunks are folded by 32 before (or 1)
 };
 
@@ -1029,6 +1053,16 @@ int launch_v(const Plan& p, const Args& a, hipStream_t st) {
   }
   const dim3 grid((unsigned)(a.B * a.nct * a.S));
   hipLaunchKernelGGL((sums_kernel<MODE, ACT, ROWS, T, V>), grid, dim3(p.nt), p.lds, st, a);
+  Args b = a;
+  b.S = p.apply_S;
+  b.per = p.apply_per;
+  const dim3 apply_grid((unsigned)(a.B * a.nct * b.S));
+  if constexpr (ROWS) {
+    if (p.fold_apply && (MODE != BWD || a.o1)) {
+      hipLaunchKernelGGL((apply_kernel<MODE, ACT, ROWS, T, V, true>), apply_grid, dim3(p.nt), p.apply_lds, st, b, a.S);
+      return hipGetLastError() == hipSuccess ? GANAMD_OK : GANAMD_ELAUNCH;
+    }
+  }
   if (p.sstep > 1) {
     typedef typename AccT<MODE>::type A;
     const int n = Sums<MODE, ACT>::K * a.C;
@@ -1037,13 +1071,8 @@ int launch_v(const Plan& p, const Args& a, hipStream_t st) {
   }
   hipLaunchKernelGGL((group_kernel<MODE, ACT>), dim3((unsigned)(a.B * ((a.G + p.gpb - 1) / p.gpb))), dim3(256),
                      MODE == FWD ? 64 * (size_t)p.gpb : 0, st, a, p.gpb, p.sstep);
-  if (MODE != BWD || a.o1) {
-    Args b = a;
-    b.S = p.apply_S;
-    b.per = p.apply_per;
-    hipLaunchKernelGGL((apply_kernel<MODE, ACT, ROWS, T, V>), dim3((unsigned)(a.B * a.nct * b.S)), dim3(p.nt), p.apply_lds,
-                       st, b);
-  }
+  if (MODE != BWD || a.o1)
+    hipLaunchKernelGGL((apply_kernel<MODE, ACT, ROWS, T, V, false>), apply_grid, dim3(p.nt), p.apply_lds, st, b, a.S);
   return hipGetLastError() == hipSuccess ? GANAMD_OK : GANAMD_ELAUNCH;
 }
 

@@ -89,6 +89,7 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     }
   }
   if (p.resident) {
+    p.fold_apply = false;
     a.S = p.apply_S = 1;
     a.per = p.apply_per = 0;
     const size_t sh = p.rows ? (size_t)gn::fold_round(K, p.V, p.nt, asz) * p.V * p.nt : (size_t)K * 16;
@@ -121,16 +122,23 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     S = std::max(S, up_to(npos, (p.rows ? 128L : 128L / p.V) * a.P));
     a.per = (int)(up_to(up_to(npos, S), a.P) * a.P);
     a.S = (int)up_to(npos, a.per);
-    // The elementwise pass: as many, while its tensors fit the 256 MB of the last-level cache; beyond,
-    // pieces in launch order, which keep what is in flight together in memory (backward of 256 such
-    // maps: 203 us with 8192 blocks, 229 with 512; of 64 maps of 64x64x64 in fp32 121 against 116).
+    // The elementwise pass: as many, while its tensors roughly fit the 256 MB of the last-level cache;
+    // well beyond it, pieces in launch order, which keep what is in flight together in memory (256
+    // maps of 64x64x96 in bf16: forward 128 us with 8192 blocks, 133 with 512, backward 203 and 229;
+    // but the 335 MB double backward of 64 maps of 64x64x64 in fp32 121 and 116).
     const long data = (mode == gn::FWD ? 2 : mode == gn::BWD ? 3 : 5) * B * L * C * esz;
-    const long SA = std::max<long>(1, std::min(up_to(data > (256L << 20) ? 8192 : 512, B * a.nct), up_to(npos, 4L * a.P)));
+    const long SA = std::max<long>(1, std::min(up_to(data > (384L << 20) ? 8192 : 512, B * a.nct), up_to(npos, 4L * a.P)));
     p.apply_per = (int)(up_to(up_to(npos, SA), a.P) * a.P);
     p.apply_S = (int)up_to(npos, p.apply_per);
     const size_t sh = p.rows ? (size_t)gn::fold_round(K, p.V, p.nt, asz) * p.V * p.nt : (size_t)K * 16;
     p.lds = std::max(asz * ((size_t)K * a.CT + sh), 4 * (size_t)tabs * a.CT);
     p.apply_lds = 4 * (size_t)tabs * a.CT;
+    // Few blocks, few chunks, all of a sample's groups in a block's reach: the elementwise blocks fold
+    // and a launch goes (64 maps of 64x64x96 in bf16 forward: 35.5 us, with a group kernel 37.5; the
+    // backward of 64 maps of 64x64x64 in fp32 69.8 against 72.8, of 7 maps of 33x31x100 15.1 against 18.5).
+    const size_t fold_lds = 64 * (size_t)G + std::max(asz * (size_t)K * C, p.apply_lds);
+    p.fold_apply = p.rows && a.nct == 1 && a.S <= 16 && B * p.apply_S <= 1024 && fold_lds <= 32 * 1024;
+    if (p.fold_apply) p.apply_lds = fold_lds;
   }
   p.gpb = (int)std::max<long>(1, std::min<long>(G, 256 / ((long)K * Cg)));
   p.sstep = a.S > 2 * gn::kFold ? gn::kFold : 1;
