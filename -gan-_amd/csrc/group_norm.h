@@ -46,7 +46,7 @@ struct Args {
   double* stats;                                // [B][G][2]: mean, r (written by FWD)
   double* coef;                                 // [B][G][8]: group coefficients of the elementwise pass
   float* part;                                  // [B][S][K][C] partial sums (FWD: doubles [B][S][2][C])
-  float* par;                                   // [3][B][C]: each sample's terms of gw, gb, gslope
+  float* par;                                   // [2 or 3][B][C]: each sample's terms of gw, gb (, gslope)
   float cslope;                                 // constant slope where slope is null
   float eps;
   long L, B;                                    // positions, samples
@@ -732,7 +732,7 @@ __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int
           sweep2<ACT>(a, q, cc + c, [&](int k) { return (double)chan[k * stride + cg + c]; }, m1, m2, terms);
           if (tell && a.par)
 #pragma unroll
-            for (int k = 0; k < 3; ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
+            for (int k = 0; k < (ACT == SLOPE ? 3 : 2); ++k) a.par[(k * a.B + b) * a.C + cc + c] = (float)terms[k];
         }
 #pragma unroll
         for (int k = 0; k < 3; ++k) m2[k] = lanes_sum(m2[k], W);

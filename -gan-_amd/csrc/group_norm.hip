@@ -144,12 +144,13 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   p.sstep = a.S > 2 * gn::kFold ? gn::kFold : 1;
   if (B * a.nct * std::max(a.S, p.apply_S) >= (1L << 31) || B * G >= (1L << 31) || p.lds > 64 * 1024) return false;
   // workspace
+  const size_t pars = p.act == gn::SLOPE ? 3 : 2;
   size_t at = 0;
   auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
   f.part = p.resident ? 0 : take(asz * (size_t)K * C * a.S * B);
   f.coef = p.resident || mode == gn::FWD ? 0 : take(64 * (size_t)B * G);
-  f.par = mode == gn::FWD ? 0 : take(4 * 3 * (size_t)B * C);
-  f.fold = mode == gn::FWD || B <= kFoldB ? 0 : take(4 * 3 * (size_t)up_to(B, kFoldB) * C);
+  f.par = mode == gn::FWD ? 0 : take(4 * pars * (size_t)B * C);
+  f.fold = mode == gn::FWD || B <= kFoldB ? 0 : take(4 * pars * (size_t)up_to(B, kFoldB) * C);
   f.total = at;
   return true;
 }

@@ -6,9 +6,11 @@
 // Here the autograd nodes are C++ and a list is read in one pass.  The kernels stay behind the C ABI
 // of include/ganamd.h; gan_amd._lib hands its entry points over (init), so one library is loaded.
 //
-// No exception leaves a function that Python calls: refused arguments become GanAmdError.
+// No exception leaves a function that Python calls: refused arguments and failed launches become
+// GanAmdError, torch's own errors (out of memory) what torch makes of them.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
@@ -22,6 +24,7 @@
 #include <cmath>
 #include <cstring>
 #include <limits>
+#include <stdexcept>
 #include <string>
 #include <vector>
 
@@ -49,8 +52,8 @@ struct Abi {
   decltype(&ganamd_adamw_clip) adamw;
 } abi = {};
 
-struct Refused {
-  std::string why;
+struct Refused : std::runtime_error {
+  using std::runtime_error::runtime_error;
 };
 
 int code(at::ScalarType t) {
@@ -60,7 +63,7 @@ int code(at::ScalarType t) {
 hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
 void done(int rc, const char* what) {
-  TORCH_CHECK(rc == GANAMD_OK, what, " failed with code ", rc);
+  if (rc != GANAMD_OK) throw Refused(std::string(what) + " failed with code " + std::to_string(rc));
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -267,7 +270,7 @@ struct Norm : torch::autograd::Function<Norm> {
 
 // ---------------------------------------------------------------------------- arguments
 const Tensor& tensor(PyObject* o, const char* what) {
-  if (!THPVariable_Check(o)) throw Refused{std::string(what) + " is a tensor; got " + Py_TYPE(o)->tp_name};
+  if (!THPVariable_Check(o)) throw Refused(std::string(what) + " is a tensor; got " + Py_TYPE(o)->tp_name);
   return THPVariable_Unpack(o);
 }
 Tensor maybe(PyObject* o, const char* what) { return o == Py_None ? Tensor() : tensor(o, what); }
@@ -275,7 +278,7 @@ double number(PyObject* o, const char* what) {
   const double v = PyFloat_Check(o) || PyLong_Check(o) ? PyFloat_AsDouble(o) : std::numeric_limits<double>::quiet_NaN();
   if ((v == -1.0 && PyErr_Occurred()) || (!PyFloat_Check(o) && !PyLong_Check(o))) {
     PyErr_Clear();
-    throw Refused{std::string(what) + " is a number"};
+    throw Refused(std::string(what) + " is a number");
   }
   return v;
 }
@@ -288,27 +291,25 @@ std::string text(PyObject* o) {
 // Runs f, a body that returns a new reference; what it throws becomes a Python error.
 template <class F>
 PyObject* guarded(const char* who, F f) {
+  HANDLE_TH_ERRORS
   try {
     return f();
   } catch (const Refused& r) {
-    PyErr_SetString(g_error, (std::string(who) + ": " + r.why).c_str());
-  } catch (const c10::Error& e) {
-    PyErr_SetString(g_error, (std::string(who) + ": " + e.what_without_backtrace()).c_str());
-  } catch (const std::exception& e) {
-    PyErr_SetString(g_error, (std::string(who) + ": " + e.what()).c_str());
-  } catch (...) {
-    PyErr_SetString(g_error, who);
+    PyErr_SetString(g_error, (std::string(who) + ": " + r.what()).c_str());
+    return nullptr;
   }
-  return nullptr;
+  END_HANDLE_TH_ERRORS
 }
 
 void arity(Py_ssize_t n, Py_ssize_t want) {
-  if (n != want) throw Refused{"takes " + std::to_string(want) + " arguments"};
+  if (n != want) throw Refused("takes " + std::to_string(want) + " arguments");
 }
 
-bool in_flat(PyObject* o) {
+// Whether t, the Python object o, is a parameter in an optimizer's flat buffer.
+bool in_flat(PyObject* o, const Tensor& t) {
   PyObject* v = nullptr;
-  if (o == Py_None || _PyObject_LookupAttr(o, g_flat_name, &v) < 0) {
+  if (!t.defined() || !t.requires_grad() || !t.is_leaf() || !t.is_contiguous()) return false;
+  if (_PyObject_LookupAttr(o, g_flat_name, &v) < 0) {
     PyErr_Clear();
     return false;
   }
@@ -328,30 +329,30 @@ PyObject* group_norm_act(PyObject*, PyObject* const* a, Py_ssize_t n) {
     d.act = act == "none" ? GANAMD_NORM_NONE : act == "silu" ? GANAMD_NORM_SILU : act == "leaky" ? GANAMD_NORM_LEAKY
           : act == "prelu" ? GANAMD_NORM_PRELU : -1;
     d.layout = layout == "nhwc" ? GANAMD_NORM_ROWS : layout == "cnhw" ? GANAMD_NORM_PLANES : -1;
-    if (d.act < 0) throw Refused{"act is none of 'none', 'silu', 'leaky', 'prelu'"};
-    if (d.layout < 0) throw Refused{"layout is neither 'nhwc' nor 'cnhw'"};
+    if (d.act < 0) throw Refused("act is none of 'none', 'silu', 'leaky', 'prelu'");
+    if (d.layout < 0) throw Refused("layout is neither 'nhwc' nor 'cnhw'");
     if (d.act == GANAMD_NORM_PRELU) {
       slope = tensor(a[5], "act='prelu': slope");
     } else if (d.act == GANAMD_NORM_LEAKY) {
       d.slope = (float)number(a[5], "act='leaky': slope");
     } else if (a[5] != Py_None) {
-      throw Refused{"act '" + act + "' takes no slope"};
+      throw Refused("act '" + act + "' takes no slope");
     }
     d.eps = (float)number(a[6], "eps");
-    if (!(d.eps > 0.f)) throw Refused{"eps is more than 0"};
-    if (!PyLong_Check(a[1]) || PyBool_Check(a[1])) throw Refused{"groups is a whole number"};
+    if (!(d.eps > 0.f)) throw Refused("eps is more than 0");
+    if (!PyLong_Check(a[1]) || PyBool_Check(a[1])) throw Refused("groups is a whole number");
     const long groups = PyLong_AsLong(a[1]);
     if (groups == -1 && PyErr_Occurred()) PyErr_Clear();
-    if (!x.is_cuda()) throw Refused{"x is on " + x.device().str()};
+    if (!x.is_cuda()) throw Refused("x is on " + x.device().str());
     d.dtype = code(x.scalar_type());
-    if (d.dtype < 0) throw Refused{std::string("x is ") + toString(x.scalar_type()) + ": float32, bfloat16 or float16"};
-    if (x.dim() < 2) throw Refused{"x has a batch and a channel dimension at least"};
+    if (d.dtype < 0) throw Refused(std::string("x is ") + toString(x.scalar_type()) + ": float32, bfloat16 or float16");
+    if (x.dim() < 2) throw Refused("x has a batch and a channel dimension at least");
     const int64_t B = d.layout == GANAMD_NORM_ROWS ? x.size(0) : x.size(1);
     const int64_t C = d.layout == GANAMD_NORM_ROWS ? x.size(-1) : x.size(0);
     if (groups < 1 || C < 1 || C % groups != 0)
-      throw Refused{std::to_string(groups) + " groups do not divide " + std::to_string(C) + " channels"};
+      throw Refused(std::to_string(groups) + " groups do not divide " + std::to_string(C) + " channels");
     const int64_t L = x.numel() ? x.numel() / (B * C) : 1;
-    if (B > INT32_MAX || C > (1 << 24) || L > (1 << 30)) throw Refused{"x is too large"};
+    if (B > INT32_MAX || C > (1 << 24) || L > (1 << 30)) throw Refused("x is too large");
     d.B = (int32_t)B;
     d.C = (int32_t)C;
     d.G = (int32_t)groups;
@@ -362,14 +363,14 @@ PyObject* group_norm_act(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (!t->defined()) continue;
       const int c = code(t->scalar_type());
       if (t->numel() != C || t->device() != x.device())
-        throw Refused{"parameters are " + std::to_string(C) + " elements each, on x's device"};
+        throw Refused("parameters are " + std::to_string(C) + " elements each, on x's device");
       if (c < 0 || (c != GANAMD_F32 && c != d.dtype) || (!first && c != d.param_dtype))
-        throw Refused{"parameters are all float32 or all of x's type"};
+        throw Refused("parameters are all float32 or all of x's type");
       d.param_dtype = c;
       first = false;
     }
-    const int64_t flat = (in_flat(a[2]) ? 1 : 0) | (in_flat(a[3]) ? 2 : 0) |
-                         (d.act == GANAMD_NORM_PRELU && in_flat(a[5]) ? 4 : 0);
+    const int64_t flat = (in_flat(a[2], w) ? 1 : 0) | (in_flat(a[3], b) ? 2 : 0) |
+                         (d.act == GANAMD_NORM_PRELU && in_flat(a[5], slope) ? 4 : 0);
     // contiguous before the node: a copy made inside it would be saved without its history
     x = x.contiguous();
     for (Tensor* t : {&w, &b, &slope})
@@ -377,7 +378,7 @@ PyObject* group_norm_act(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (x.numel()) {                   // refuses what the kernels cannot take, before anything runs
       size_t need = 0;
       for (int op = 0; op < 3; ++op)
-        if (abi.norm_workspace(&d, op, &need) != GANAMD_OK) throw Refused{"x is too large"};
+        if (abi.norm_workspace(&d, op, &need) != GANAMD_OK) throw Refused("x is too large");
     }
     const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     bool grad = x.requires_grad();
@@ -393,25 +394,25 @@ PyObject* group_norm_act(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // One tensor of the list `name`; throws what is wrong with it.
 const Tensor& member(PyObject* o, const char* name, int& device) {
   const std::string what(name);
-  if (!THPVariable_Check(o)) throw Refused{what + " are tensors; got " + Py_TYPE(o)->tp_name};
+  if (!THPVariable_Check(o)) throw Refused(what + " are tensors; got " + Py_TYPE(o)->tp_name);
   const Tensor& t = THPVariable_Unpack(o);
-  if (t.layout() != at::kStrided) throw Refused{what + " are dense tensors"};
-  if (!t.is_cuda()) throw Refused{what + " are on one GPU; got one on " + t.device().str()};
+  if (t.layout() != at::kStrided) throw Refused(what + " are dense tensors");
+  if (!t.is_cuda()) throw Refused(what + " are on one GPU; got one on " + t.device().str());
   if (device < 0) device = t.get_device();
-  if (t.get_device() != device) throw Refused{what + " are on one GPU; got several"};
+  if (t.get_device() != device) throw Refused(what + " are on one GPU; got several");
   if (code(t.scalar_type()) < 0)
-    throw Refused{what + " are float32, bfloat16 or float16; got " + toString(t.scalar_type())};
-  if (!t.is_non_overlapping_and_dense()) throw Refused{what + " are stored densely, each element once"};
+    throw Refused(what + " are float32, bfloat16 or float16; got " + toString(t.scalar_type()));
+  if (!t.is_non_overlapping_and_dense()) throw Refused(what + " are stored densely, each element once");
   return t;
 }
 
 // The table of the list `ts` and its outputs `outs` (a null pointer: none of their own).
 std::vector<ganamd_tensor> table(PyObject* ts, PyObject* outs, bool writes, Tensor& like) {
-  if (!PyList_Check(ts) || (outs && !PyList_Check(outs))) throw Refused{"lists of tensors are wanted"};
+  if (!PyList_Check(ts) || (outs && !PyList_Check(outs))) throw Refused("lists of tensors are wanted");
   const Py_ssize_t n = PyList_GET_SIZE(ts);
   if (outs && PyList_GET_SIZE(outs) != n)
-    throw Refused{std::to_string(n) + " gradients, " + std::to_string(PyList_GET_SIZE(outs)) + " outputs"};
-  if (n > INT32_MAX) throw Refused{"too many tensors"};
+    throw Refused(std::to_string(n) + " gradients, " + std::to_string(PyList_GET_SIZE(outs)) + " outputs");
+  if (n > INT32_MAX) throw Refused("too many tensors");
   std::vector<ganamd_tensor> rows((size_t)n);
   int device = -1;
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -419,13 +420,13 @@ std::vector<ganamd_tensor> table(PyObject* ts, PyObject* outs, bool writes, Tens
     const Tensor* o = &t;
     if (outs) {
       o = &member(PyList_GET_ITEM(outs, i), "outputs", device);
-      if (o->numel() != t.numel()) throw Refused{"an output has another number of elements than its gradient"};
+      if (o->numel() != t.numel()) throw Refused("an output has another number of elements than its gradient");
       if (!(t.is_contiguous() && o->is_contiguous()) && t.strides() != o->strides())
-        throw Refused{"a gradient that is not contiguous needs an output of its own strides"};
+        throw Refused("a gradient that is not contiguous needs an output of its own strides");
       if (o->scalar_type() != t.scalar_type() && o->scalar_type() != at::kFloat)
-        throw Refused{"an output is of its gradient's type or float32"};
+        throw Refused("an output is of its gradient's type or float32");
     }
-    if (writes && o->requires_grad()) throw Refused{"writes into a tensor that requires a gradient (detach it)"};
+    if (writes && o->requires_grad()) throw Refused("writes into a tensor that requires a gradient (detach it)");
     ganamd_tensor& r = rows[(size_t)i];
     r.p = t.const_data_ptr();
     r.out = const_cast<void*>(o->const_data_ptr());
@@ -444,7 +445,7 @@ PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::NoGradGuard plain;
     Tensor like;
     const auto rows = table(a[0], nullptr, false, like);
-    if (rows.empty()) throw Refused{"no tensors"};
+    if (rows.empty()) throw Refused("no tensors");
     const c10::DeviceGuard guard(like.device());
     const Tensor norm = at::empty({}, like.options().dtype(at::kFloat));
     const size_t need = abi.grad_workspace(rows.data(), (int)rows.size());
@@ -463,7 +464,7 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::NoGradGuard plain;
     Tensor like;
     const auto rows = table(a[0], a[1] == Py_None ? nullptr : a[1], true, like);
-    if (rows.empty()) throw Refused{"no tensors"};
+    if (rows.empty()) throw Refused("no tensors");
     const float most = (float)number(a[2], "max_norm");
     const c10::DeviceGuard guard(like.device());
     const Tensor norm = at::empty({}, like.options().dtype(at::kFloat));
@@ -471,8 +472,13 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor ws = scratch(need, like);
     const int rc = abi.grad_clip(rows.data(), (int)rows.size(), (int)PyLong_AsLong(a[3]), most, norm.data_ptr<float>(),
                                  ptr(ws), need, stream_of(like));
-    if (rc == GANAMD_EINVAL) throw Refused{"tensors that are written to share memory with others of the call"};
+    if (rc == GANAMD_EINVAL) throw Refused("tensors that are written to share memory with others of the call");
     done(rc, "grad_clip");
+    PyObject* written = a[1] == Py_None ? a[0] : a[1];
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(written); ++i) {     // autograd sees that they changed
+      const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(written, i));
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
     return THPVariable_Wrap(norm);
   });
 }
@@ -487,28 +493,28 @@ PyObject* clipped_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (int i = 0; i < 4; ++i) {
       t[i] = tensor(a[i], names[i]);
       if (!t[i].is_cuda() || t[i].scalar_type() != at::kFloat || !t[i].is_contiguous())
-        throw Refused{std::string(names[i]) + " is a contiguous float32 tensor on the GPU"};
-      if (t[i].numel() != t[0].numel()) throw Refused{std::string(names[i]) + " has another number of elements than param"};
+        throw Refused(std::string(names[i]) + " is a contiguous float32 tensor on the GPU");
+      if (t[i].numel() != t[0].numel()) throw Refused(std::string(names[i]) + " has another number of elements than param");
     }
     const Tensor& step = tensor(a[4], "step");
     if (!step.is_cuda() || step.scalar_type() != at::kInt || step.numel() != 1)
-      throw Refused{"step is one int32 on the GPU"};
+      throw Refused("step is one int32 on the GPU");
     double k[5];
     const char* nums[5] = {"lr", "beta1", "beta2", "eps", "weight_decay"};
     for (int i = 0; i < 5; ++i) k[i] = number(a[5 + i], nums[i]);
     const float most = (float)number(a[10], "max_norm");
-    if (!(most >= 0.f)) throw Refused{"max_norm is 0 or more"};
+    if (!(most >= 0.f)) throw Refused("max_norm is 0 or more");
     const int64_t count = t[0].numel();
     for (int i = 0; i < 4; ++i) {
-      if (t[i].device() != step.device()) throw Refused{"the buffers and the counter are on one device"};
+      if (t[i].device() != step.device()) throw Refused("the buffers and the counter are on one device");
       for (int j = 0; j < i && count; ++j) {
         const auto p = reinterpret_cast<uintptr_t>(t[i].data_ptr()), q = reinterpret_cast<uintptr_t>(t[j].data_ptr());
-        if (p < q + 4 * count && q < p + 4 * count) throw Refused{"four separate buffers are wanted"};
+        if (p < q + 4 * count && q < p + 4 * count) throw Refused("four separate buffers are wanted");
       }
     }
     Tensor norm = maybe(a[11], "norm");
     if (norm.defined() && (norm.device() != step.device() || norm.scalar_type() != at::kFloat || norm.numel() != 1))
-      throw Refused{"norm is one float32 on the buffers' device"};
+      throw Refused("norm is one float32 on the buffers' device");
     const c10::DeviceGuard guard(step.device());
     if (!norm.defined()) norm = at::empty({}, step.options().dtype(at::kFloat));
     if (count) {

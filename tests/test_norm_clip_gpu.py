@@ -320,6 +320,42 @@ def test_penalty_step_with_group_norm_and_clip(act):
             assert float((u.detach().double().cpu() - q[k].detach()).abs().max()) < 4e-4 * 1e-3 + 2.0 ** -22, k
 
 
+@pytest.mark.parametrize("shape,G,layout,dtype", [((64, 64, 64, 24), 4, "nhwc", BF16), ((24, 64, 64, 64), 3, "cnhw", F32),
+                                                  ((256, 64, 64, 24), 8, "nhwc", F16)])
+def test_group_norm_large(ops, shape, G, layout, dtype):
+    """Whole batches of full-size maps, up to and beyond the last-level cache: statistics and gradients
+    by their sums (the tested quantities are linear or quadratic in the outputs)."""
+    t = make(shape, layout, "leaky", dtype, 21)
+    x, w, b = (t[k].detach().requires_grad_() for k in ("x", "w", "b"))
+    y = ops.group_norm_act(x, G, w, b, act="leaky", slope=0.2, layout=layout)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], t["gy"])
+    xd, gyd = t["x"].double(), t["gy"].double()
+    if layout == "cnhw":
+        xd, gyd, yd, gxd = (u.permute(1, 2, 3, 0) for u in (xd, gyd, y.double(), gx.double()))
+    else:
+        yd, gxd = y.double(), gx.double()
+    B, C = xd.shape[0], xd.shape[-1]
+    grp = lambda u: u.reshape(B, -1, G, C // G)   # noqa: E731
+    d = grp(xd) - grp(xd).mean((1, 3), keepdim=True)
+    r = 1 / torch.sqrt((d * d).mean((1, 3), keepdim=True) + 1e-5)
+    wd, bd = (u.detach().double().reshape(1, 1, G, C // G) for u in (w, b))
+    z = d * r * wd + bd
+    a1 = torch.where(z > 0, 1.0, 0.2).double()
+    half = HALF[dtype]
+    err = (grp(yd) - z * a1).abs()
+    assert bool((err <= (half + 2.0 ** -16) * ((z - bd).abs() + bd.abs()) + TINY[dtype]).all())
+    u = grp(gyd) * a1 * wd
+    xh = d * r
+    m1, m2 = u.mean((1, 3), keepdim=True), (u * xh).mean((1, 3), keepdim=True)
+    ref = r * (u - m1 - xh * m2)
+    mag = r * (u.abs() + u.abs().mean((1, 3), keepdim=True) * (1 + xh.abs()))
+    assert bool(((grp(gxd) - ref).abs() <= (half + 2.0 ** -16) * mag + TINY[dtype]).all())
+    g = grp(gyd) * a1
+    for got, want, size in ((gw, g * xh, g.abs() * xh.abs()), (gb, g, g.abs())):
+        lim = 2.0 ** -16 * size.sum((0, 1)).reshape(C)
+        assert bool(((got.double() - want.sum((0, 1)).reshape(C)).abs() <= lim).all())
+
+
 def test_group_norm_third_derivative_is_refused(ops):
     t = make((2, 4, 8), "nhwc", "silu", F32, 19)
     x, gy = (t[k].detach().requires_grad_() for k in ("x", "gy"))
@@ -615,6 +651,45 @@ def test_clip_and_step_graph(ops):
         assert all(torch.equal(a, b) for a, b in zip(want, outs))
         n = ops.clipped_adamw_(state[0], g, state[1], state[2], state[3], *k)
         assert torch.equal(n, nb) and all(torch.equal(a, b) for a, b in zip(state, (p, m, v, step)))
+
+
+def test_clip_counts_as_a_write(ops):
+    """A tensor that autograd saved and the clip scaled is noticed."""
+    t = torch.randn(50, device=DEV)
+    w = torch.randn(50, device=DEV, requires_grad=True)
+    y = (w * t).sum()
+    ops.clip_grad_norm_([t], 0.1)
+    with pytest.raises(RuntimeError, match="modified"):
+        y.backward()
+
+
+def test_optimizer_step_graph(ops):
+    """FusedAdamW(max_grad_norm) captured and replayed; the norm is the replay's."""
+    from gan_amd.optim import FusedAdamW
+    a, b = (torch.nn.Linear(53, 31).to(DEV) for _ in range(2))
+    b.load_state_dict(a.state_dict())
+    oa, ob = FusedAdamW(a, max_grad_norm=0.5), FusedAdamW(b, max_grad_norm=0.5)
+    g = [torch.randn(oa.flat.n_train, generator=torch.Generator().manual_seed(i)).to(DEV) for i in range(4)]
+    for o in (oa, ob):                       # one eager step each, on a side stream
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            o.flat.grad.copy_(g[0])
+            o.step()
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ob.step()
+    for i in range(1, 4):
+        oa.flat.grad.copy_(g[i])
+        ob.flat.grad.copy_(g[i])
+        oa.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(oa.flat.data, ob.flat.data) and torch.equal(oa.grad_norm, ob.grad_norm)
+        assert abs(float(ob.grad_norm) - float(g[i].double().norm())) <= 2.0 ** -23 * float(g[i].double().norm())
+        assert int(ob.step_count) == i + 1
 
 
 def test_clip_other_stream_and_repeats(ops):
