@@ -55,6 +55,7 @@ struct Args {
   int CT, nct;                                  // channels per tile, tiles
   int S;                                        // chunks of a sample's positions
   int per;                                      // positions (planes: vectors) per chunk
+  bool once;                                    // outputs go past the caches
 };
 
 // ------------------------------------------------------------------ types
@@ -151,7 +152,7 @@ __device__ __forceinline__ Vec<T, V> load(const T* p) {
   return v;
 }
 template <class T, int V>
-__device__ __forceinline__ void store(T* p, const Vec<T, V>& v, int skip) {
+__device__ __forceinline__ void store(T* p, const Vec<T, V>& v, int skip, bool once) {
   typedef typename Vec<T, V>::W W;
   if (skip == 0) {
     W x;
@@ -159,7 +160,13 @@ __device__ __forceinline__ void store(T* p, const Vec<T, V>& v, int skip) {
       x = (W)v.w[0];
     else
       __builtin_memcpy(&x, v.w, sizeof(x));
-    *reinterpret_cast<W*>(p) = x;
+    if (once) {
+      asm volatile("");                 // (else the two stores become one, without the hint)
+      __builtin_nontemporal_store(x, reinterpret_cast<W*>(p));
+      asm volatile("");
+    } else {
+      *reinterpret_cast<W*>(p) = x;
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -747,8 +754,8 @@ __device__ __forceinline__ void write(const Args& a, const Lin<MODE, ACT> (&ln)[
                                       const Vec<T, V>& x, const Vec<T, V>& gy, const Vec<T, V>& v) {
   Vec<T, V> o1, o2;
   apply<MODE, ACT, ROWS, T, V, NC>(ln, x, gy, v, o1, o2);
-  if (MODE != BWD || a.o1) store(static_cast<T*>(a.o1) + at, o1, skip);
-  if constexpr (MODE == DBL) store(static_cast<T*>(a.o2) + at, o2, skip);
+  if (MODE != BWD || a.o1) store(static_cast<T*>(a.o1) + at, o1, skip, a.once);
+  if constexpr (MODE == DBL) store(static_cast<T*>(a.o2) + at, o2, skip, a.once);
 }
 
 // ------------------------------------------------------------------ the resident form

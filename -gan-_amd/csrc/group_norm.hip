@@ -58,6 +58,13 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   const long few = mode == gn::DBL ? 4 : 8;
   a.L = L; a.B = B; a.C = C; a.G = G; a.Cg = Cg; a.eps = d->eps; a.pdt = d->param_dtype;
   a.cslope = d->act == GANAMD_NORM_LEAKY ? d->slope : 1.f;
+  // A call whose tensors are well beyond the 256 MB of the last-level cache: its outputs are stored past
+  // the caches (forward and a copy of its output, 256 maps of 64x64x96 in bf16: 190 us against 212;
+  // for smaller ones the call itself gains too, but the kernel that reads its output loses as much:
+  // 64 maps of 64x64x64 in fp32 with the copy 69 against 67).
+  const long data = (mode == gn::FWD ? 2 : mode == gn::BWD ? 3 : 5) * B * L * C * esz;
+  const bool large = data >= (384L << 20);
+  a.once = large;
   p.resident = false;
   const long nv = up_to(L, p.V);
   if (p.rows) {
@@ -122,12 +129,10 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     S = std::max(S, up_to(npos, (p.rows ? 128L : 128L / p.V) * a.P));
     a.per = (int)(up_to(up_to(npos, S), a.P) * a.P);
     a.S = (int)up_to(npos, a.per);
-    // The elementwise pass: as many, while its tensors roughly fit the 256 MB of the last-level cache;
-    // well beyond it, pieces in launch order, which keep what is in flight together in memory (256
-    // maps of 64x64x96 in bf16: forward 128 us with 8192 blocks, 133 with 512, backward 203 and 229;
-    // but the 335 MB double backward of 64 maps of 64x64x64 in fp32 121 and 116).
-    const long data = (mode == gn::FWD ? 2 : mode == gn::BWD ? 3 : 5) * B * L * C * esz;
-    const long SA = std::max<long>(1, std::min(up_to(data > (384L << 20) ? 8192 : 512, B * a.nct), up_to(npos, 4L * a.P)));
+    // The elementwise pass: as many; for large calls pieces in launch order, which keep what is in flight
+    // together in memory (the same maps: forward 128 us with 8192 blocks, 133 with 512, backward 203
+    // and 229; but the 335 MB double backward of 64 maps of 64x64x64 in fp32 121 and 116).
+    const long SA = std::max<long>(1, std::min(up_to(large ? 8192 : 512, B * a.nct), up_to(npos, 4L * a.P)));
     p.apply_per = (int)(up_to(up_to(npos, SA), a.P) * a.P);
     p.apply_S = (int)up_to(npos, p.apply_per);
     const size_t sh = p.rows ? (size_t)gn::fold_round(K, p.V, p.nt, asz) * p.V * p.nt : (size_t)K * 16;
