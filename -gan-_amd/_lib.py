@@ -26,10 +26,7 @@ EPI_STORE, EPI_BIAS, EPI_DEMOD, EPI_ACCUM, EPI_SCALE = 0, 1, 2, 3, 4
 CONV_FWD, CONV_DGRAD, CONV_WGRAD = 0, 1, 2
 ACT_SIGMOID, ACT_TANH, ACT_LEAKY = 0, 1, 2
 MATH_F32, MATH_BF16 = 0, 1
-F32, BF16, F16 = 0, 1, 2                                # element types (GANAMD_F32 ...)
-NORM_ROWS, NORM_PLANES = 0, 1                           # ganamd_norm_desc.layout
-NORM_NONE, NORM_SILU, NORM_LEAKY, NORM_PRELU = 0, 1, 2, 3   # ganamd_norm_desc.act
-NORM_L2, NORM_MAX = 0, 1                                # kinds of gradient norm
+NORM_L2, NORM_MAX = 0, 1     # kinds of gradient norm
 KERNEL_PATCH_FWD, KERNEL_PATCH_DGRAD, KERNEL_WGRAD_ROW, KERNEL_SMALL = 1, 2, 4, 8   # ganamd_conv_desc.kernel_off bits
 
 
