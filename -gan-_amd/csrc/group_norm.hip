@@ -147,7 +147,9 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   }
   p.gpb = (int)std::max<long>(1, std::min<long>(G, 256 / ((long)K * Cg)));
   p.sstep = a.S > 2 * gn::kFold ? gn::kFold : 1;
-  if (B * a.nct * std::max(a.S, p.apply_S) >= (1L << 31) || B * G >= (1L << 31) || p.lds > 64 * 1024) return false;
+  if (B * a.nct * std::max(a.S, p.apply_S) >= (1L << 31) || B * G >= (1L << 31) || p.lds > 64 * 1024 ||
+      up_to(B, kFoldB) > 65535)
+    return false;
   // workspace
   const size_t pars = p.act == gn::SLOPE ? 3 : 2;
   size_t at = 0;
@@ -207,7 +209,6 @@ int fold_params(const Full& f, char* ws, int K, void* gw, void* gb, void* gs, in
   if (B > kFoldB) {
     float* mid = reinterpret_cast<float*>(ws + f.fold);
     const long nc = up_to(B, kFoldB);
-    if (nc > 65535) return GANAMD_EINVAL;
     hipLaunchKernelGGL(param_kernel, dim3(gx, K, (unsigned)nc), dim3(1024), 0, st, in, B, C, kFoldB, mid, gw, gb, gs, dt, 0);
     in = mid;
     B = nc;

@@ -180,7 +180,8 @@ def test_group_norm_abi_refusals():
     assert L.ganamd_group_norm_workspace(_lib.NormDesc(**good), 1, n) == 0 and n.value > 0
     need = n.value
     for bad in (dict(L=0), dict(B=0), dict(C=0), dict(G=0), dict(G=3), dict(layout=2), dict(dtype=3),
-                dict(param_dtype=-1), dict(act=4), dict(eps=0.0), dict(eps=float("nan")), dict(L=1 << 31)):
+                dict(param_dtype=-1), dict(act=4), dict(eps=0.0), dict(eps=float("nan")), dict(L=1 << 31),
+                dict(B=65535 * 512 + 1)):
         assert L.ganamd_group_norm_workspace(_lib.NormDesc(**{**good, **bad}), 0, n) == -1, bad
     d = _lib.NormDesc(**good)
     assert L.ganamd_group_norm_workspace(d, 3, n) == -1 and L.ganamd_group_norm_workspace(d, -1, n) == -1

@@ -356,6 +356,70 @@ def test_group_norm_large(ops, shape, G, layout, dtype):
         assert bool(((got.double() - want.sum((0, 1)).reshape(C)).abs() <= lim).all())
 
 
+@pytest.mark.parametrize("layout", ["nhwc", "cnhw"])
+def test_group_norm_offsets_beyond_32_bits(ops, layout):
+    """2.2e9 elements: the last sample alone gives the same, to its rounding."""
+    B, H, C = 530, 64, 1024
+    shape = (B, H, H, C) if layout == "nhwc" else (C, B, H, H)
+    x = torch.empty(shape, dtype=BF16, device=DEV).normal_(0.5, 2.0)
+    gy = torch.empty(shape, dtype=BF16, device=DEV).normal_()
+    w, b = torch.full((C,), 1.25, device=DEV), torch.full((C,), -0.1, device=DEV)
+    xl = x.requires_grad_()
+    y = ops.group_norm_act(xl, 32, w, b, act="silu", layout=layout)
+    (gx,) = torch.autograd.grad(y, xl, gy)
+    last = (slice(-1, None),) if layout == "nhwc" else (slice(None), slice(-1, None))
+    t = {k: u[last].detach().contiguous() for k, u in (("x", x), ("gy", gy))}
+    ref = reference(t["x"], 32, w, b, "silu", None, 1e-5, layout, t["gy"])
+    close(y[last].contiguous(), ref["y"], "y")
+    close(gx[last].contiguous(), ref["gx"], "gx")
+
+
+def test_group_norm_samples_beyond_16_bits(ops):
+    for shape, layout in (((70_001, 8), "nhwc"), ((8, 70_001), "cnhw")):
+        check_all(ops, make(shape, layout, "prelu", F32, 22), 2, "prelu", layout)
+
+
+def test_two_streams_at_once(ops):
+    """Norms and clips on two streams, issued in turn: neither disturbs the other."""
+    ts = [make((6, 40, 40, 24), "nhwc", "prelu", F32, 30 + i) for i in range(2)]
+    gs = [grads([5, 70_000, 300] * 60, [F32], 40 + i) for i in range(2)]
+    want = [run_all(ops, t, 3, "prelu", "nhwc") for t in ts]
+    outs = [[torch.empty_like(t) for t in g] for g in gs]
+    norms = [ops.clip_grad_norm_(g, 0.01, out=o) for g, o in zip(gs, outs)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got, again, ns = [None] * 2, [[torch.empty_like(t) for t in g] for g in gs], [None] * 2
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = run_all_quiet(ops, ts[i])
+                ns[i] = ops.clip_grad_norm_(gs[i], 0.01, out=again[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, k in zip(got[i], ("y", "gx", "gw")):
+            assert torch.equal(a, want[i][k])
+        assert torch.equal(ns[i], norms[i]) and all(torch.equal(a, b) for a, b in zip(again[i], outs[i]))
+
+
+def run_all_quiet(ops, t):
+    """Forward and backward without a look at the results in between."""
+    x, w = (t[k].detach().requires_grad_() for k in ("x", "w"))
+    y = ops.group_norm_act(x, 3, w, t["b"], act="prelu", slope=t["slope"])
+    return [y, *torch.autograd.grad(y, [x, w], t["gy"])]
+
+
+def test_clip_offsets_beyond_32_bits(ops):
+    t = torch.empty(1_300_000_001, device=DEV).normal_()
+    n = float(torch.linalg.vector_norm(t, dtype=torch.float64))
+    tail = t[-1000:].clone()
+    out = torch.empty_like(t)
+    got = ops.clip_grad_norm_([t[:7], t[7:]], 0.5 * n, out=[out[:7], out[7:]])
+    assert abs(float(got) - n) <= 2.0 ** -22 * n
+    c = 0.5 * n / (n + 1e-6)
+    assert bool(((out[-1000:].double() - tail.double() * c).abs() <= tail.double().abs() * 4 * 2.0 ** -24).all())
+
+
 def test_group_norm_third_derivative_is_refused(ops):
     t = make((2, 4, 8), "nhwc", "silu", F32, 19)
     x, gy = (t[k].detach().requires_grad_() for k in ("x", "gy"))
