@@ -187,14 +187,14 @@ struct NormBackward : torch::autograd::Function<NormBackward> {
       if (wanted >> i & 1) {
         gg[i] = grads[k++];
         any = any || gg[i].defined();
-        if (gg[i].defined()) gg[i] = gg[i].contiguous();
+        if (gg[i].defined()) gg[i] = gg[i].detach().to(par[i].scalar_type()).contiguous();
       }
     if (!any) return none;
     const bool differentiable = at::GradMode::is_enabled();
     variable_list out(9);
     {
       const at::NoGradGuard plain;
-      ggx = ggx.defined() ? ggx.contiguous() : at::zeros_like(x);
+      ggx = ggx.defined() ? ggx.to(x.scalar_type()).contiguous() : at::zeros_like(x);
       bool want[3];
       asked(ctx, 2, par, want);
       const Targets t = targets(par, want, differentiable ? 0 : flat);
@@ -246,7 +246,7 @@ struct Norm : torch::autograd::Function<Norm> {
     const Tensor &x = s[0], &stats = s[4];
     const Tensor par[3] = {s[1], s[2], s[3]};
     const int64_t flat = ctx->saved_data["flat"].toInt();
-    const Tensor gy = grads[0].contiguous();
+    const Tensor gy = grads[0].to(x.scalar_type()).contiguous();
     bool want[3];
     asked(ctx, 1, par, want);
     variable_list out(6);

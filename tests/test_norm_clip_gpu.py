@@ -205,6 +205,15 @@ def test_group_norm_many_samples(ops):
     check_all(ops, make((24, 1300), "cnhw", "silu", F32, 15), 4, "silu", "cnhw")
 
 
+def test_group_norm_gradient_of_another_type(ops):
+    """A float32 cotangent of a bf16 result is taken in the result's type."""
+    t = make((3, 6, 5, 16), "nhwc", "silu", BF16, 23)
+    x = t["x"].clone().requires_grad_()
+    y = ops.group_norm_act(x, 4, t["w"], t["b"], act="silu")
+    want = torch.autograd.grad(y, x, t["gy"], retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(y, x, t["gy"].float())[0], want)
+
+
 def test_group_norm_one_sided_gradients(ops):
     """Some inputs without a gradient: the others' do not change."""
     t = make((3, 6, 5, 16), "nhwc", "prelu", F32, 16)
@@ -354,6 +363,25 @@ def test_group_norm_large(ops, shape, G, layout, dtype):
     for got, want, size in ((gw, g * xh, g.abs() * xh.abs()), (gb, g, g.abs())):
         lim = 2.0 ** -16 * size.sum((0, 1)).reshape(C)
         assert bool(((got.double() - want.sum((0, 1)).reshape(C)).abs() <= lim).all())
+
+
+MANY_CHUNKS = [((1, 200_000, 8), 2, "nhwc"), ((1, 90_001, 3), 3, "nhwc"), ((2, 1, 1_200_001), 1, "cnhw"),
+               ((1, 1, 2_000_000), 1, "cnhw")]
+
+
+@pytest.mark.parametrize("shape,G,layout", MANY_CHUNKS)
+@pytest.mark.parametrize("dtype,act", [(F32, "prelu"), (BF16, "silu")])
+def test_group_norm_many_chunks(ops, shape, G, layout, dtype, act):
+    """One long sample over so many chunks that they are folded in two steps."""
+    import ctypes
+    from gan_amd import _lib
+    B, C = (shape[0], shape[-1]) if layout == "nhwc" else (shape[1], shape[0])
+    d = _lib.NormDesc(math.prod(shape) // (B * C), B, C, G, ("nhwc", "cnhw").index(layout), (F32, BF16).index(dtype), 0,
+                      3 if act == "prelu" else 1, 0.0, 1e-5)
+    for op in range(3):
+        info = (ctypes.c_int * 11)()
+        assert _lib.LIB.ganamd_group_norm_plan_info(d, op, info) == 0 and not info[0] and info[7] > 64
+    check_all(ops, make(shape, layout, act, dtype, 24), G, act, layout)
 
 
 @pytest.mark.parametrize("layout", ["nhwc", "cnhw"])
