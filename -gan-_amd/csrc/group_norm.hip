@@ -76,7 +76,7 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     if (gt * Cg < p.V) gt = G;
     const long CT = gt * Cg, TX = up_to(CT, p.V);
     if (TX <= most) {
-      const long P = std::min(most / TX, std::max(up_to(L, few), std::min(L, up_to(256, TX))));
+      const long P = std::min(most / TX, std::max(up_to(L, few), std::min(L, 256 / TX)));
       const long R = up_to(L, P), nct = up_to(G, gt);
       if (R <= rcap && (R <= 2 || B * nct >= 96)) {
         p.resident = true;
