@@ -6,6 +6,7 @@
 set -e
 cd "$(dirname "$0")/.."
 mkdir -p tools/variants
+FLAGS=$(python3 -c "import __graft_entry__ as e; print(*e.FLAGS)")   # the in-tree build's
 P=./-gan-_amd
 U=${UNIT:-conv_gemm}
 SRC=$P/csrc/$U.hip
@@ -13,10 +14,10 @@ if [ -n "$3" ]; then
   SRC=$P/csrc/.ab_rev_$U.hip
   git show "$3:-gan-_amd/csrc/$U.hip" > "$SRC"
 fi
-/opt/rocm/bin/hipcc -O3 --offload-arch=gfx950 -std=c++17 -fPIC $2 -c $SRC -o tools/variants/$1.o
+/opt/rocm/bin/hipcc $FLAGS $2 -c $SRC -o tools/variants/$1.o
 [ -n "$3" ] && rm -f "$SRC"
 OBJS=""
-for u in conv_gemm conv_patch conv_wgrad_row conv_small elem gemm_grouped fused data act rng critic; do
+for u in $(python3 -c "import __graft_entry__ as e, os; print(*[os.path.basename(s)[:-4] for s in e.SOURCES])"); do
   [ "$u" = "$U" ] || OBJS="$OBJS $P/build/$u.hip.o"
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -fPIC -shared -o tools/variants/$1.so tools/variants/$1.o $OBJS
