@@ -127,6 +127,8 @@ Targets targets(const Tensor* par, const bool* want, int64_t flat) {
       const auto it = info->find(node.get());
       if (it != info->end() && it->second.captures_) all = false;
     }
+    // one parameter in two places: its two sums are added by different blocks, so not into one buffer
+    for (int j = 0; j < i; ++j) all = all && !(want[j] && par[j].defined() && par[j].const_data_ptr() == par[i].const_data_ptr());
   }
   t.flat = any && all;
   for (int i = 0; i < 3; ++i)

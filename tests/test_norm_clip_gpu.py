@@ -492,6 +492,32 @@ def test_group_norm_flat_gradients(ops):
         assert torch.equal(p.grad, g)
 
 
+def test_group_norm_one_parameter_in_two_places(ops):
+    """A parameter of a flat buffer that is weight and bias at once: the sum of both gradients arrives."""
+    from gan_amd.optim import FusedAdamW
+    D = Block().to(DEV)
+    FusedAdamW(D)
+    t = make((8, 3, 6, 6), "cnhw", "silu", F32, 18)
+    free = [D.gamma.detach().clone().requires_grad_() for _ in range(2)]
+    for order in (1, 2):
+        D._flat.grad.zero_()
+        got = []
+        for w, b in ((D.gamma, D.gamma), free):
+            x = t["x"].clone().requires_grad_()
+            y = ops.group_norm_act(x, 2, w, b, act="silu", layout="cnhw")
+            if order == 2:
+                (gx,) = torch.autograd.grad(y, x, t["gy"], create_graph=True)
+                y, up = gx, t["v"]
+            else:
+                up = t["gy"]
+            if w is b:
+                y.backward(up)
+            else:
+                got = torch.autograd.grad(y, free, up)
+        assert torch.equal(D.gamma.grad, got[0] + got[1])
+        assert D.gamma.grad.data_ptr() >= D._flat.grad.data_ptr()
+
+
 def test_group_norm_graph(ops):
     """Forward, backward and double backward captured; replays with eager work between them."""
     for shape, G, layout in (((2, 9, 9, 12), 3, "nhwc"), ((1, 3000, 8), 2, "nhwc"), ((12, 2, 37), 3, "cnhw")):
