@@ -128,7 +128,8 @@ Targets targets(const Tensor* par, const bool* want, int64_t flat) {
       if (it != info->end() && it->second.captures_) all = false;
     }
     // one parameter in two places: its two sums are added by different blocks, so not into one buffer
-    for (int j = 0; j < i; ++j) all = all && !(want[j] && par[j].defined() && par[j].const_data_ptr() == par[i].const_data_ptr());
+    for (int j = 0; j < i; ++j)
+      if (want[j] && par[j].const_data_ptr() == par[i].const_data_ptr()) all = false;
   }
   t.flat = any && all;
   for (int i = 0; i < 3; ++i)
@@ -440,6 +441,11 @@ std::vector<ganamd_tensor> table(PyObject* ts, PyObject* outs, bool writes, Tens
   return rows;
 }
 
+// Counts a write into t: autograd notices it in a tensor it saved, the packed copies of a weight that they are stale.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // grad_norm(tensors, kind) of a list that is not empty
 PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded("grad_norm", [&]() -> PyObject* {
@@ -476,11 +482,8 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                  ptr(ws), need, stream_of(like));
     if (rc == GANAMD_EINVAL) throw Refused("tensors that are written to share memory with others of the call");
     done(rc, "grad_clip");
-    PyObject* written = a[1] == Py_None ? a[0] : a[1];
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(written); ++i) {     // autograd sees that they changed
-      const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(written, i));
-      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-    }
+    PyObject* outs = a[1] == Py_None ? a[0] : a[1];
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(outs); ++i) written(THPVariable_Unpack(PyList_GET_ITEM(outs, i)));
     return THPVariable_Wrap(norm);
   });
 }
@@ -517,6 +520,13 @@ PyObject* clipped_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Tensor norm = maybe(a[11], "norm");
     if (norm.defined() && (norm.device() != step.device() || norm.scalar_type() != at::kFloat || norm.numel() != 1))
       throw Refused("norm is one float32 on the buffers' device");
+    const void* small[2] = {step.const_data_ptr(), norm.defined() ? norm.const_data_ptr() : nullptr};
+    for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < 4 && count; ++j) {
+        const auto p = reinterpret_cast<uintptr_t>(small[i]), q = reinterpret_cast<uintptr_t>(t[j].data_ptr());
+        if (p < q + 4 * count && q < p + 4) throw Refused("step and norm lie outside the buffers");
+      }
+    if (small[0] == small[1]) throw Refused("step and norm are two tensors");
     const c10::DeviceGuard guard(step.device());
     if (!norm.defined()) norm = at::empty({}, step.options().dtype(at::kFloat));
     if (count) {
@@ -530,6 +540,7 @@ PyObject* clipped_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
       norm.zero_();
       step.add_(1);
     }
+    for (const Tensor* w : {&t[0], &t[2], &t[3]}) written(*w);
     return THPVariable_Wrap(norm);
   });
 }

@@ -1584,5 +1584,5 @@ def clipped_adamw_(param, grad, exp_avg, exp_avg_sq, step, lr, betas, eps, weigh
     """One AdamW step (``FusedAdamW``) of a flat float32 buffer on its gradient clipped to the global
     norm ``max_norm``: ``param``, ``exp_avg``, ``exp_avg_sq`` and the int32 device counter ``step``
     are updated in place, ``grad`` stays unscaled.  Returns the norm (0-dim float32 on the device;
-    ``norm``: a tensor to write it into).  Two launches, no host synchronisation."""
+    ``norm``: a tensor to write it into).  The six share no memory.  Two launches, no host synchronisation."""
     return _lib.HOST.clipped_adamw(param, grad, exp_avg, exp_avg_sq, step, lr, *betas, eps, weight_decay, max_norm, norm)

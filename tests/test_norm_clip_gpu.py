@@ -781,6 +781,32 @@ def test_clip_counts_as_a_write(ops):
         y.backward()
 
 
+def test_clipped_adamw_counts_as_a_write(ops):
+    """A convolution after a step on its weight uses the new weight, not the packed copy of the old."""
+    w = torch.nn.Parameter(torch.randn(8, 8, 3, 3, generator=torch.Generator().manual_seed(1)).to(DEV))
+    x = torch.randn(8, 2, 16, 16, generator=torch.Generator().manual_seed(2)).to(DEV)
+    geo = ops.conv_geo(2, 8, 16, 16, 8, 3, 1, 1)
+    conv = lambda w: ops.conv2d(x, w, None, geo, 1.0)   # noqa: E731
+    old = conv(w).detach()
+    step = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.clipped_adamw_(w.detach(), torch.ones_like(w), torch.zeros_like(w), torch.zeros_like(w), step, 0.1, (0.9, 0.99),
+                       1e-8, 0.0, 1.0)
+    new = conv(w).detach()
+    assert not torch.equal(old, new)
+    assert torch.equal(new, conv(torch.nn.Parameter(w.detach().clone())).detach())
+
+
+def test_clipped_adamw_refuses_overlaps(ops):
+    from gan_amd._lib import GanAmdError
+    p, g, m, v = (torch.ones(64, device=DEV) for _ in range(4))
+    step = torch.zeros(1, dtype=torch.int32, device=DEV)
+    k = (1e-3, (0.9, 0.999), 1e-8, 0.01, 1.0)
+    for bad in (dict(norm=p[3]), dict(norm=g[63:]), dict(norm=step.view(F32)), dict(step=v[5:6].view(torch.int32))):
+        with pytest.raises(GanAmdError):
+            ops.clipped_adamw_(p, g, m, v, bad.get("step", step), *k, norm=bad.get("norm"))
+    assert int(step) == 0 and all(bool((t == 1).all()) for t in (p, g, m, v))
+
+
 def test_optimizer_step_graph(ops):
     """FusedAdamW(max_grad_norm) captured and replayed; the norm is the replay's."""
     from gan_amd.optim import FusedAdamW
