@@ -157,6 +157,34 @@ void asked(AutogradContext* ctx, int first, const Tensor* par, bool* want) {
   for (int i = 0; i < 3; ++i) want[i] = par[i].defined() && ctx->needs_input_grad(e++);
 }
 
+// Whether a gradient that `node` hands on along edge e goes to a node of the default stream from
+// another one.  The engine makes that stream wait for this one, which no capture allows: while a graph
+// is captured, its error comes where nothing catches it and ends the process.
+bool leaves_for_default_stream(torch::autograd::Node& node, size_t e) {
+  const auto& edges = node.next_edges();
+  if (e >= edges.size() || !edges[e].is_valid()) return false;
+  const auto from = node.stream(), to = edges[e].function->stream();
+  return from && to && *from != *to && to->id() == 0;
+}
+
+// Refuses a backward under capture whose gradients would leave the capture: what an eager graph of the
+// same leaves, still alive, makes of it.  Edges from `first` on are the parameters'; gradients that are
+// added to a flat buffer go nowhere.
+void stay_in_capture(AutogradContext* ctx, int first, bool flat, const Tensor& like) {
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const size_t n = node->next_edges().size();
+  bool leaves = false;
+  for (size_t e = 0; e < n; ++e)
+    if (ctx->needs_input_grad(e) && !(flat && e >= (size_t)first)) leaves = leaves || leaves_for_default_stream(*node, e);
+  if (!leaves) return;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream_of(like), &status) != hipSuccess) throw Refused("hipStreamIsCapturing failed");
+  if (status != hipStreamCaptureStatusNone)
+    throw Refused("group_norm_act: a backward in a graph capture reaches what was recorded eagerly on the default "
+                  "stream (delete the eager results that share its inputs before the capture)");
+}
+
 // (gx, gradients of the wanted parameters) as a function of (gy, x, w, b, slope): what a backward
 // with create_graph makes, differentiable once more.
 struct NormBackward : torch::autograd::Function<NormBackward> {
@@ -201,6 +229,7 @@ struct NormBackward : torch::autograd::Function<NormBackward> {
       bool want[3];
       asked(ctx, 2, par, want);
       const Targets t = targets(par, want, differentiable ? 0 : flat);
+      stay_in_capture(ctx, 2, t.flat, x);
       const Tensor g_gy = at::empty_like(x), g_x = at::empty_like(x);
       if (x.numel()) {
         const c10::DeviceGuard guard(x.device());
@@ -254,6 +283,7 @@ struct Norm : torch::autograd::Function<Norm> {
     asked(ctx, 1, par, want);
     variable_list out(6);
     if (at::GradMode::is_enabled()) {
+      stay_in_capture(ctx, 1, false, x);
       const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
       const int64_t wanted = want[0] | want[1] << 1 | want[2] << 2;
       const variable_list g =
@@ -264,6 +294,7 @@ struct Norm : torch::autograd::Function<Norm> {
       return out;
     }
     const Targets t = targets(par, want, flat);
+    stay_in_capture(ctx, 1, t.flat, x);
     if (ctx->needs_input_grad(0)) out[0] = at::empty_like(x);
     norm_backward(d, gy, x, par, stats, out[0], t);
     for (int i = 0; i < 3 && !t.flat; ++i) out[1 + i] = t.g[i];
@@ -545,6 +576,16 @@ PyObject* clipped_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// Whether the node that made the tensor hands a gradient to the default stream from another one.
+PyObject* crosses(PyObject*, PyObject* o) {
+  return guarded("crosses", [&]() -> PyObject* {
+    const auto node = tensor(o, "y").grad_fn();
+    bool yes = false;
+    for (size_t e = 0; node && e < node->next_edges().size(); ++e) yes = yes || leaves_for_default_stream(*node, e);
+    return PyBool_FromLong(yes);
+  });
+}
+
 // init(GanAmdError, {entry point: address})
 PyObject* init(PyObject*, PyObject* args) {
   PyObject *error = nullptr, *where = nullptr;
@@ -581,6 +622,7 @@ PyMethodDef methods[] = {
     {"grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(grad_norm)), METH_FASTCALL, nullptr},
     {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(clip)), METH_FASTCALL, nullptr},
     {"clipped_adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(clipped_adamw)), METH_FASTCALL, nullptr},
+    {"crosses", crosses, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

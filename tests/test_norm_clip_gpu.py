@@ -518,6 +518,57 @@ def test_group_norm_one_parameter_in_two_places(ops):
         assert D.gamma.grad.data_ptr() >= D._flat.grad.data_ptr()
 
 
+def test_group_norm_backward_that_leaves_a_capture_is_refused(ops):
+    """A captured backward into leaves that an eager graph of the default stream holds is refused before
+    it runs; once that graph is gone, it is captured and replays."""
+    from gan_amd._lib import HOST
+    t = make((4, 8, 5, 5), "cnhw", "silu", F32, 19)
+    x = t["x"].clone().requires_grad_()
+    w, b = (t[k].detach().clone().requires_grad_() for k in "wb")
+    call = lambda: ops.group_norm_act(x, 2, w, b, act="silu", layout="cnhw")   # noqa: E731
+    want = torch.autograd.grad(call(), (x, w, b), t["gy"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = call()
+        assert not HOST.crosses(y)
+        del y
+    eager = call()
+    assert not HOST.crosses(eager)
+    with torch.cuda.stream(side):
+        y = call()
+        assert HOST.crosses(y)
+        for u, v in zip(torch.autograd.grad(y, (x, w, b), t["gy"]), want):      # no capture: no refusal
+            assert torch.equal(u, v)
+        del y
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call()
+        assert HOST.crosses(y)
+        for again in (False, True):
+            with pytest.raises(RuntimeError, match="capture"):
+                torch.autograd.grad(y, (x, w, b), t["gy"], create_graph=again, retain_graph=True)
+        kept = t["gy"] * 2
+        del y
+    del eager
+    torch.cuda.synchronize()
+    other = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other):
+        y = call()
+        assert not HOST.crosses(y)
+        got = torch.autograd.grad(y, (x, w, b), t["gy"])
+        del y
+    for _ in range(3):
+        for g in got:
+            g.fill_(float("nan"))
+        graph.replay()
+        other.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(kept, t["gy"] * 2) and all(torch.equal(g, u) for g, u in zip(got, want))
+
+
 def test_group_norm_graph(ops):
     """Forward, backward and double backward captured; replays with eager work between them."""
     for shape, G, layout in (((2, 9, 9, 12), 3, "nhwc"), ((1, 3000, 8), 2, "nhwc"), ((12, 2, 37), 3, "cnhw")):
