@@ -192,16 +192,11 @@ def _plain(s):
         p -= size * (m / (torch.sqrt(v) / root + ADAM_EPS))
         return dict(p=p, m=m, v=v, step=s["step"], norm=norm.float())
     if op == "clip":
-        _, outs = _clip_types(case)
+        ins, _ = _clip_types(case)
         flat = torch.cat([t.float() for t in s["grads"]])
         norm = torch.sqrt((flat.double() * flat.double()).sum())
         flat *= torch.clamp(s["limit"] / (norm + CLIP_EPS), max=1.0).float()
-        pieces = flat.split([t.numel() for t in s["grads"]])
-        if len(s["dst"]) == 1:
-            torch._foreach_copy_(s["targets"], list(pieces))
-        else:                             # (it takes destinations of one type only)
-            for t, buf in s["dst"].items():
-                buf.copy_(torch.cat([p for p, u in zip(pieces, outs) if u == t]))
+        torch._foreach_copy_(s["targets"], list(flat.split([t.numel() for t in s["grads"]])))
         return dict(norm=norm.float(), **s["dst"])
     dt = s["x"].dtype
     x = s["x"].float()
