@@ -303,9 +303,17 @@ struct Norm : torch::autograd::Function<Norm> {
 };
 
 // ---------------------------------------------------------------------------- arguments
+
+// No operator here pushes tangents forward.  A dual tensor does not require a gradient, so it would
+// be taken as its primal and its tangent lost without a word.
+void no_tangent(const Tensor& t, const char* what) {
+  if (t._fw_grad(/*level=*/0).defined()) throw Refused(std::string(what) + ": a forward-mode tangent (not supported)");
+}
 const Tensor& tensor(PyObject* o, const char* what) {
   if (!THPVariable_Check(o)) throw Refused(std::string(what) + " is a tensor; got " + Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  no_tangent(t, what);
+  return t;
 }
 Tensor maybe(PyObject* o, const char* what) { return o == Py_None ? Tensor() : tensor(o, what); }
 double number(PyObject* o, const char* what) {
@@ -430,6 +438,7 @@ const Tensor& member(PyObject* o, const char* name, int& device) {
   const std::string what(name);
   if (!THPVariable_Check(o)) throw Refused(what + " are tensors; got " + Py_TYPE(o)->tp_name);
   const Tensor& t = THPVariable_Unpack(o);
+  no_tangent(t, name);
   if (t.layout() != at::kStrided) throw Refused(what + " are dense tensors");
   if (!t.is_cuda()) throw Refused(what + " are on one GPU; got one on " + t.device().str());
   if (device < 0) device = t.get_device();
@@ -526,8 +535,8 @@ PyObject* clipped_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::NoGradGuard plain;
     const char* names[4] = {"param", "grad", "exp_avg", "exp_avg_sq"};
     Tensor t[4];
+    for (int i = 0; i < 4; ++i) t[i] = tensor(a[i], names[i]);
     for (int i = 0; i < 4; ++i) {
-      t[i] = tensor(a[i], names[i]);
       if (!t[i].is_cuda() || t[i].scalar_type() != at::kFloat || !t[i].is_contiguous())
         throw Refused(std::string(names[i]) + " is a contiguous float32 tensor on the GPU");
       if (t[i].numel() != t[0].numel()) throw Refused(std::string(names[i]) + " has another number of elements than param");

@@ -1523,7 +1523,8 @@ def group_norm_act(x, groups: int, weight=None, bias=None, act: str = "none", sl
     ReLU), ``"prelu"`` (``slope``: ``[C]``, with a gradient).  Parameters are all float32 or all of
     x's type, as are their gradients; the arithmetic is float32, statistics float64.  Gradients of
     parameters in an optimizer's flat buffer are added there by the kernel.
-    A non-contiguous ``x`` is copied first; an empty one gives an empty result.  A backward under
+    A non-contiguous ``x`` is copied first; an empty one gives an empty result.  Forward-mode
+    derivatives are refused.  A backward under
     graph capture whose inputs an eager result on the default stream still holds is refused
     (delete that result first)."""
     return _lib.HOST.group_norm_act(x, groups, weight, bias, act, slope, eps, layout)

@@ -269,3 +269,23 @@ def test_trainers_and_optimizer_take_max_grad_norm():
     tr = mk(rng=object(), max_grad_norm=2.0)
     assert tr.optimizer_G.max_grad_norm == tr.optimizer_D.max_grad_norm == 2.0
     assert mk(rng=object()).optimizer_D.max_grad_norm is None
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent is never dropped silently, whichever argument carries it."""
+    import torch.autograd.forward_ad as fwad
+    from gan_amd import _lib, ops
+    x, w = torch.zeros(2, 3, 3, 8), torch.ones(8)
+    step = torch.zeros(1, dtype=torch.int32)
+    b = [torch.zeros(8) for _ in range(4)]
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))   # noqa: E731
+        for f in (lambda: ops.group_norm_act(dual(x), 2, w, w), lambda: ops.group_norm_act(x, 2, dual(w), w),
+                  lambda: ops.group_norm_act(x, 2, w, dual(w)), lambda: ops.grad_norm([dual(w)]),
+                  lambda: ops.group_norm_act(x, 2, w, w, act="prelu", slope=dual(w)),
+                  lambda: ops.clip_grad_norm_([dual(w)], 1.0),
+                  lambda: ops.clipped_adamw_(b[0], dual(b[1]), *b[2:], step, 1e-3, (0.9, 0.999), 1e-8, 0.0, 1.0)):
+            with torch.no_grad(), pytest.raises(_lib.GanAmdError, match="tangent"):
+                f()
+            with pytest.raises(_lib.GanAmdError, match="tangent"):
+                f()

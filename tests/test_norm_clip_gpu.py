@@ -897,3 +897,18 @@ def test_clip_other_stream_and_repeats(ops):
         k = ops.clip_grad_norm_(ts, 0.02, out=b)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(n, k) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_forward_mode_is_refused_on_the_gpu(ops):
+    import torch.autograd.forward_ad as fwad
+    from gan_amd._lib import GanAmdError
+    t = make((2, 4, 4, 8), "nhwc", "prelu", F32, 33)
+    with fwad.dual_level():
+        dual = lambda u: fwad.make_dual(u, torch.ones_like(u))   # noqa: E731
+        for k in ("x", "w", "b", "slope"):
+            a = {**t, k: dual(t[k])}
+            with pytest.raises(GanAmdError, match="tangent"):
+                ops.group_norm_act(a["x"], 2, a["w"], a["b"], act="prelu", slope=a["slope"])
+        for f in (ops.grad_norm, lambda u: ops.clip_grad_norm_(u, 1.0)):
+            with pytest.raises(GanAmdError, match="tangent"):
+                f([t["x"], dual(t["gy"])])
