@@ -102,7 +102,10 @@ Tensor norm_forward(const ganamd_norm_desc& d, const Tensor& x, const Tensor& w,
 
 // Where the gradients of w, b and slope go: new tensors; or, where every wanted one is of a
 // parameter in a flat buffer and this is a first-order backward, the buffer's views themselves
-// (added to; the engine then gets none).
+// (added to; the engine then gets none).  The engine orders streams along the gradients that it is
+// handed, so that takes the parameters' accumulators on the running node's own stream: what adds to
+// them there, and who waits for that stream after the backward, is then in order.  (They are on another
+// one where a parameter is used on two streams, or where an older graph of it still lives.)
 struct Targets {
   Tensor g[3];
   bool flat = false;
@@ -110,7 +113,8 @@ struct Targets {
 
 Targets targets(const Tensor* par, const bool* want, int64_t flat) {
   Targets t;
-  bool any = false, all = !at::GradMode::is_enabled();
+  const auto self = torch::autograd::get_current_node();
+  bool any = false, all = self && !at::GradMode::is_enabled();
   for (int i = 0; i < 3; ++i) {
     if (!want[i]) continue;
     any = true;
@@ -123,6 +127,7 @@ Targets targets(const Tensor* par, const bool* want, int64_t flat) {
     // a gradient that autograd.grad was asked for is returned, not added
     const auto node = torch::autograd::impl::try_get_grad_accumulator(par[i]);
     const auto* info = torch::autograd::get_current_graph_task_exec_info();
+    all = all && node && node->stream() == self->stream();
     if (node && info) {
       const auto it = info->find(node.get());
       if (it != info->end() && it->second.captures_) all = false;
@@ -168,15 +173,14 @@ bool leaves_for_default_stream(torch::autograd::Node& node, size_t e) {
 }
 
 // Refuses a backward under capture whose gradients would leave the capture: what an eager graph of the
-// same leaves, still alive, makes of it.  Edges from `first` on are the parameters'; gradients that are
-// added to a flat buffer go nowhere.
-void stay_in_capture(AutogradContext* ctx, int first, bool flat, const Tensor& like) {
+// same leaves, still alive, makes of it.
+void stay_in_capture(AutogradContext* ctx, const Tensor& like) {
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
   const size_t n = node->next_edges().size();
   bool leaves = false;
   for (size_t e = 0; e < n; ++e)
-    if (ctx->needs_input_grad(e) && !(flat && e >= (size_t)first)) leaves = leaves || leaves_for_default_stream(*node, e);
+    if (ctx->needs_input_grad(e)) leaves = leaves || leaves_for_default_stream(*node, e);
   if (!leaves) return;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(stream_of(like), &status) != hipSuccess) throw Refused("hipStreamIsCapturing failed");
@@ -229,7 +233,7 @@ struct NormBackward : torch::autograd::Function<NormBackward> {
       bool want[3];
       asked(ctx, 2, par, want);
       const Targets t = targets(par, want, differentiable ? 0 : flat);
-      stay_in_capture(ctx, 2, t.flat, x);
+      stay_in_capture(ctx, x);
       const Tensor g_gy = at::empty_like(x), g_x = at::empty_like(x);
       if (x.numel()) {
         const c10::DeviceGuard guard(x.device());
@@ -283,7 +287,7 @@ struct Norm : torch::autograd::Function<Norm> {
     asked(ctx, 1, par, want);
     variable_list out(6);
     if (at::GradMode::is_enabled()) {
-      stay_in_capture(ctx, 1, false, x);
+      stay_in_capture(ctx, x);
       const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
       const int64_t wanted = want[0] | want[1] << 1 | want[2] << 2;
       const variable_list g =
@@ -294,7 +298,7 @@ struct Norm : torch::autograd::Function<Norm> {
       return out;
     }
     const Targets t = targets(par, want, flat);
-    stay_in_capture(ctx, 1, t.flat, x);
+    stay_in_capture(ctx, x);
     if (ctx->needs_input_grad(0)) out[0] = at::empty_like(x);
     norm_backward(d, gy, x, par, stats, out[0], t);
     for (int i = 0; i < 3 && !t.flat; ++i) out[1 + i] = t.g[i];

@@ -1522,7 +1522,8 @@ def group_norm_act(x, groups: int, weight=None, bias=None, act: str = "none", sl
     None (ones / zeros).  ``act``: ``"none"``, ``"silu"``, ``"leaky"`` (``slope``: a number; 0 is a
     ReLU), ``"prelu"`` (``slope``: ``[C]``, with a gradient).  Parameters are all float32 or all of
     x's type, as are their gradients; the arithmetic is float32, statistics float64.  Gradients of
-    parameters in an optimizer's flat buffer are added there by the kernel.
+    parameters in an optimizer's flat buffer are added there by the kernel, where the backward runs on
+    the stream that the parameters' accumulators belong to (else autograd adds them).
     A non-contiguous ``x`` is copied first; an empty one gives an empty result.  Forward-mode
     derivatives are refused.  A backward under
     graph capture whose inputs an eager result on the default stream still holds is refused

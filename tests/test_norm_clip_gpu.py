@@ -912,3 +912,113 @@ def test_forward_mode_is_refused_on_the_gpu(ops):
         for f in (ops.grad_norm, lambda u: ops.clip_grad_norm_(u, 1.0)):
             with pytest.raises(GanAmdError, match="tangent"):
                 f([t["x"], dual(t["gy"])])
+
+
+def flat_case(ops, seed, act="prelu"):
+    """A Block with its flat buffer, data, the call, and what one backward adds to the norm's parameters."""
+    from gan_amd.optim import FusedAdamW
+    D = Block(act=act).to(DEV)
+    FusedAdamW(D)
+    t = make((8, 3, 6, 6), "cnhw", act, F32, seed)
+    pars = (D.gamma, D.beta, D.slope)
+    call = lambda x: ops.group_norm_act(x, 2, D.gamma, D.beta, act=act, slope=D.slope, layout="cnhw")   # noqa: E731
+    free = [p.detach().clone().requires_grad_() for p in pars]
+    y = ops.group_norm_act(t["x"], 2, free[0], free[1], act=act, slope=free[2], layout="cnhw")
+    want = torch.autograd.grad(y, free, t["gy"])
+    torch.cuda.synchronize()
+    return D, t, pars, call, want
+
+
+def sleep():
+    torch.cuda._sleep(20_000_000)       # about 10 ms: what does not wait for this stream is seen
+
+
+def test_group_norm_flat_gradients_of_two_streams(ops):
+    """One module on the default and on a side stream, one backward: both gradients arrive, and the
+    caller's stream waits for them."""
+    D, t, pars, call, want = flat_case(ops, 34)
+    side = torch.cuda.Stream()
+    for late in (0, 1):
+        for first in (0, 1):                       # which stream makes the accumulators
+            D._flat.grad.zero_()
+            side.wait_stream(torch.cuda.current_stream())
+            ys = [None, None]
+            for i in (first, 1 - first):
+                with torch.cuda.stream(side) if i else torch.cuda.stream(torch.cuda.current_stream()):
+                    ys[i] = call(t["x"])
+            with torch.cuda.stream(side) if late else torch.cuda.stream(torch.cuda.current_stream()):
+                sleep()
+            torch.autograd.backward(ys, [t["gy"], t["gy"]])
+            got = [p.grad.clone() for p in pars]
+            del ys
+            for g, w in zip(got, want):
+                assert torch.equal(g, w + w)
+            assert all(p.grad.data_ptr() >= D._flat.grad.data_ptr() for p in pars)
+
+
+@pytest.mark.parametrize("order", [1, 2])
+def test_group_norm_flat_gradients_beside_a_living_graph(ops, order):
+    """The parameters' accumulators are those of an eager graph of the default stream; the call runs on
+    a side stream and x needs no gradient: the caller's stream still waits for the side stream's add."""
+    D, t, pars, call, want = flat_case(ops, 35)
+    older = call(t["x"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x = t["x"].clone().requires_grad_(order == 2)
+        y, up = call(x), t["gy"]
+        if order == 2:
+            (y,), up = torch.autograd.grad(y, x, t["gy"], create_graph=True), t["v"]
+        sleep()
+    y.backward(up, inputs=list(pars))
+    got = [p.grad.clone() for p in pars]
+    torch.cuda.synchronize()
+    del older, y
+    if order == 2:
+        x = t["x"].clone().requires_grad_()
+        D._flat.grad.zero_()
+        (gx,) = torch.autograd.grad(call(x), x, t["gy"], create_graph=True)
+        gx.backward(t["v"], inputs=list(pars))
+        want = [p.grad.clone() for p in pars]
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+
+
+def test_group_norm_flat_gradients_of_a_side_stream(ops):
+    """All on one side stream: added by the kernel there, and the caller's stream waits for it."""
+    D, t, pars, call, want = flat_case(ops, 36)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = call(t["x"])
+        sleep()
+    y.backward(t["gy"])
+    for p, w in zip(pars, want):
+        assert torch.equal(p.grad.clone(), w)
+
+
+def test_group_norm_flat_gradients_captured(ops):
+    """A captured backward adds to the flat buffer on every replay; beside a living eager graph of the
+    default stream, whose accumulators no capture can reach, it is refused."""
+    D, t, pars, call, want = flat_case(ops, 37)
+    D._flat.grad.zero_()
+    older = call(t["x"])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture"):
+            call(t["x"]).backward(t["gy"])
+    del older
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(t["x"]).backward(t["gy"])
+    torch.cuda.synchronize()
+    assert not D._flat.grad.any()
+    total = [torch.zeros_like(w) for w in want]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        total = [a + w for a, w in zip(total, want)]
+        for p, a in zip(pars, total):
+            assert torch.equal(p.grad, a)
