@@ -389,7 +389,7 @@ bool plan(const ganamd_tensor* l, int n, Plan& p) {
   while (p.chunk < kChunkMax && total / p.chunk > 2048) p.chunk *= 2;
   p.chunks = 0;
   for (int i = 0; i < n; ++i) p.chunks += (l[i].n + p.chunk - 1) / p.chunk;
-  if (p.chunks >= (1L << 31)) return false;
+  if (p.chunks * kNT >= (1L << 32)) return false;      // threads of a launch
   p.entries = sizeof(double) * ((size_t)p.chunks + 1);
   p.owner = p.entries + (p.tensors > kTable ? sizeof(Entry) * (size_t)p.tensors : 0);
   p.total = p.owner + (p.tensors > kTable ? sizeof(uint32_t) * (size_t)p.chunks : 0);
@@ -543,7 +543,7 @@ int ganamd_adamw_clip(float* p, const float* g, float* m, float* v, long n, int3
                       double beta2, double eps, double weight_decay, float max_norm, float* norm, void* workspace,
                       size_t workspace_bytes, hipStream_t st) {
   const long blocks = std::max<long>(1, (n / 4 + kNT * kStepVec - 1) / (kNT * kStepVec));
-  if (!p || !g || !m || !v || !step || !norm || n <= 0 || blocks >= (1L << 31) || !(max_norm >= 0.f) || !workspace ||
+  if (!p || !g || !m || !v || !step || !norm || n <= 0 || blocks * kNT >= (1L << 32) || !(max_norm >= 0.f) || !workspace ||
       workspace_bytes < ganamd_adamw_clip_workspace())
     return GANAMD_EINVAL;
   double* part = static_cast<double*>(workspace);

@@ -147,8 +147,12 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   }
   p.gpb = (int)std::max<long>(1, std::min<long>(G, 256 / ((long)K * Cg)));
   p.sstep = a.S > 2 * gn::kFold ? gn::kFold : 1;
-  if (B * a.nct * std::max(a.S, p.apply_S) >= (1L << 31) || B * G >= (1L << 31) || p.lds > 64 * 1024 ||
-      up_to(B, kFoldB) > 65535)
+  // A launch holds fewer than 2^32 threads across x and 2^16 blocks across y or z; the kernels' block numbers
+  // are 32 bits.  (In doubles: the products of absurd sizes pass 64 bits.)
+  const double blocks = (double)B * a.nct * std::max(a.S, p.apply_S), most_threads = 4294967295.0;
+  if (blocks >= 2147483648.0 || blocks * p.nt > most_threads || (double)B * G >= 2147483648.0 || p.lds > 64 * 1024 ||
+      up_to(B, kFoldB) > 65535 || (p.sstep > 1 && B > 65535) ||
+      (!p.resident && (double)B * up_to(G, p.gpb) * 256 > most_threads))
     return false;
   // workspace
   const size_t pars = p.act == gn::SLOPE ? 3 : 2;

@@ -421,15 +421,16 @@ PyObject* group_norm_act(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x = x.contiguous();
     for (Tensor* t : {&w, &b, &slope})
       if (t->defined()) *t = t->contiguous();
+    bool grad = x.requires_grad();
+    for (const Tensor* t : {&w, &b, &slope}) grad = grad || (t->defined() && t->requires_grad());
+    grad = grad && at::GradMode::is_enabled();
     if (x.numel()) {                   // refuses what the kernels cannot take, before anything runs
       size_t need = 0;
-      for (int op = 0; op < 3; ++op)
+      for (int op = 0; op < (grad ? 3 : 1); ++op)
         if (abi.norm_workspace(&d, op, &need) != GANAMD_OK) throw Refused("x is too large");
     }
     const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-    bool grad = x.requires_grad();
-    for (const Tensor* t : {&w, &b, &slope}) grad = grad || (t->defined() && t->requires_grad());
-    if (grad && at::GradMode::is_enabled()) return THPVariable_Wrap(Norm::apply(x, opt(w), opt(b), opt(slope), d, flat));
+    if (grad) return THPVariable_Wrap(Norm::apply(x, opt(w), opt(b), opt(slope), d, flat));
     const at::NoGradGuard plain;
     Tensor stats;
     return THPVariable_Wrap(norm_forward(d, x, w, b, slope, stats));

@@ -289,3 +289,32 @@ def test_forward_mode_is_refused():
                 f()
             with pytest.raises(_lib.GanAmdError, match="tangent"):
                 f()
+
+
+@pytest.mark.parametrize("L,C,G,layout,dtype", [(1, 1024, 32, 0, 0), (1, 1024, 32, 0, 1), (1, 96, 32, 0, 0), (1, 8, 2, 1, 0),
+                                                (2048, 2048, 4, 0, 1), (40_000, 4, 2, 1, 0), (5, 1, 1, 0, 2)])
+@pytest.mark.parametrize("op", [0, 1, 2])
+def test_plan_refuses_what_no_launch_holds(L, C, G, layout, dtype, op):
+    """The largest batch that is taken needs fewer than 2^32 threads in every launch over the maps; one
+    sample more would not, unless the limit of 65535 * 512 samples comes first."""
+    from gan_amd import _lib
+
+    def threads(B):
+        d = _lib.NormDesc(L, B, C, G, layout, dtype, 0, 1, 0.0, 1e-5)
+        info, n = (ctypes.c_int * 11)(), _lib.c_size_t(0)
+        rc = _lib.LIB.ganamd_group_norm_plan_info(d, op, info)
+        assert rc == _lib.LIB.ganamd_group_norm_workspace(d, op, n)
+        return None if rc else B * info[6] * max(info[7], info[9]) * info[2]
+
+    lo, hi = 1, 65535 * 512 + 1
+    assert threads(lo) and threads(hi) is None
+    while hi - lo > 1:
+        mid = (lo + hi) // 2
+        if threads(mid) is None:
+            hi = mid
+        else:
+            lo = mid
+    assert threads(lo) < 1 << 32
+    assert lo == 65535 * 512 or threads(lo) * hi // lo >= 1 << 32
+    for B in (2_100_000, 4_200_000, 33_000_000):
+        assert threads(B) is None or threads(B) < 1 << 32
