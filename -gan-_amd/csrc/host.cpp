@@ -585,7 +585,7 @@ PyObject* clipped_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
       norm.zero_();
       step.add_(1);
     }
-    for (const Tensor* w : {&t[0], &t[2], &t[3]}) written(*w);
+    for (const Tensor& w : {t[0], t[2], t[3], step, norm}) written(w);
     return THPVariable_Wrap(norm);
   });
 }

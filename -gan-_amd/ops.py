@@ -199,9 +199,10 @@ class PackCache:
     """GEMM-order copies of parameter weights, reused by every conv call on the same weight
     (forward, input-gradient backward, the gradient penalty's double backward) until the weight
     changes.  A weight changes through (a) the fused optimizer, which bumps the epoch of its flat
-    buffer (``FlatParams.epoch``; parameters outside one follow the global ``invalidate()``), or
+    buffer (``FlatParams.epoch``; parameters outside one follow the global ``invalidate()``),
     (b) torch in-place ops on the Parameter (``load_state_dict``, ``p.copy_``), which bump its
-    version counter.  Only weights that are Parameters (or views of one) are cached.
+    version counter, or (c) writes to the flat buffer itself (``clipped_adamw_`` on it, torch in-place
+    ops), which bump the buffer's version counter and not the Parameters'.  Only weights that are Parameters (or views of one) are cached.
 
     Weights living in an optimizer's flat buffer get a PERSISTENT copy (allocated eagerly, kept
     for the life of the model) registered with that buffer (``PackRegistry``): the optimizer
@@ -248,7 +249,7 @@ class PackCache:
                     return e.packed
                 if cap == 0:          # reloaded / modified in place: refresh this copy now
                     cls._pack(geo, op, w, e.packed)
-                    e.version, e.epoch = root._version, flat.epoch
+                    e.version, e.epoch, e.data_version = root._version, flat.epoch, flat.data._version
                     return e.packed
             elif cap == 0:            # first use: a persistent copy, refreshed by the optimizer
                 packed = cls._alloc(geo, op, w)
@@ -259,7 +260,7 @@ class PackCache:
         # it: eager code, or ONE graph capture (its buffer lives in that graph's memory and is
         # refreshed only when that graph replays).
         key = base_key + (cap,)
-        epoch = (id(flat), flat.epoch) if flat is not None else cls.epoch
+        epoch = (id(flat), flat.epoch, flat.data._version) if flat is not None else cls.epoch
         e = cls.entries.get(key)
         if e is not None and e[0]() is root and e[1] == root._version and e[2] == epoch:
             return e[3]
@@ -273,10 +274,11 @@ class PackCache:
 
 
 class _PackEntry:
-    __slots__ = ("root", "version", "epoch", "packed", "job")
+    __slots__ = ("root", "version", "epoch", "data_version", "packed", "job")
 
-    def __init__(self, root, version, epoch, packed, job):
-        self.root, self.version, self.epoch, self.packed, self.job = root, version, epoch, packed, job
+    def __init__(self, root, version, epoch, data_version, packed, job):
+        self.root, self.version, self.epoch, self.data_version = root, version, epoch, data_version
+        self.packed, self.job = packed, job
 
 
 class PackRegistry:
@@ -295,11 +297,12 @@ class PackRegistry:
     def add(self, key, root, geo, op, w, packed, epoch):
         job = _lib.PackJob()
         check(LIB.ganamd_conv_pack_job(geo.desc(), op, ptr(w), ptr(packed), job), "conv_pack_job")
-        self.entries[key] = _PackEntry(root, root._version, epoch, packed, job)
+        self.entries[key] = _PackEntry(root, root._version, epoch, self.flat.data._version, packed, job)
         self.dirty = True
 
     def valid(self, e) -> bool:
-        return e.epoch == self.flat.epoch or (self.batch_epoch == self.flat.epoch and e.epoch <= self.batch_epoch)
+        return (e.data_version == self.flat.data._version and
+                (e.epoch == self.flat.epoch or (self.batch_epoch == self.flat.epoch and e.epoch <= self.batch_epoch)))
 
     def repack(self):
         """After the optimizer update (flat.epoch already bumped): refresh every copy, one launch."""
@@ -324,7 +327,7 @@ class PackRegistry:
               "conv_pack_batch")
         self.batch_epoch = self.flat.epoch
         for e in self.entries.values():       # every copy now reflects the current weights
-            e.version, e.epoch = e.root._version, self.flat.epoch
+            e.version, e.epoch, e.data_version = e.root._version, self.flat.epoch, self.flat.data._version
 
 
 def invalidate_packed():
@@ -1588,5 +1591,8 @@ def clipped_adamw_(param, grad, exp_avg, exp_avg_sq, step, lr, betas, eps, weigh
     """One AdamW step (``FusedAdamW``) of a flat float32 buffer on its gradient clipped to the global
     norm ``max_norm``: ``param``, ``exp_avg``, ``exp_avg_sq`` and the int32 device counter ``step``
     are updated in place, ``grad`` stays unscaled.  Returns the norm (0-dim float32 on the device;
-    ``norm``: a tensor to write it into).  The six share no memory.  Two launches, no host synchronisation."""
+    ``norm``: a tensor to write it into).  The six share no memory.  Two launches, no host synchronisation.
+    Counts as an in-place write to what it updates: convolutions repack weights that lie in ``param``
+    (an optimizer's flat buffer too) at their next eager call.  Inside or between captured graphs use
+    ``FusedAdamW.step``, which refreshes the packed copies itself."""
     return _lib.HOST.clipped_adamw(param, grad, exp_avg, exp_avg_sq, step, lr, *betas, eps, weight_decay, max_norm, norm)

@@ -1022,3 +1022,33 @@ def test_group_norm_flat_gradients_captured(ops):
         total = [a + w for a, w in zip(total, want)]
         for p, a in zip(pars, total):
             assert torch.equal(p.grad, a)
+
+
+def test_clipped_adamw_on_a_flat_buffer_counts_as_a_write(ops):
+    """A convolution of a parameter in an optimizer's flat buffer, after the buffer itself was updated
+    (by the op or by torch), uses the new weight; the optimizer's own step leaves its copies valid."""
+    from gan_amd.optim import FusedAdamW
+    D = Block().to(DEV)
+    opt = FusedAdamW(D, max_grad_norm=1.0)
+    f, n = opt.flat, opt.flat.n_train
+    x = torch.randn(3, 2, 16, 16, generator=torch.Generator().manual_seed(2)).to(DEV)
+    geo = ops.conv_geo(2, 3, 16, 16, 8, 3, 1, 1)
+    conv = lambda w: ops.conv2d(x, w, None, geo, 1.0).detach()   # noqa: E731
+    fresh = lambda: conv(torch.nn.Parameter(D.w0.detach().clone()))   # noqa: E731
+    step, norm = torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros((), device=DEV)
+    m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    old = conv(D.w0)
+    assert f.packs.entries
+    for write in (lambda: ops.clipped_adamw_(f.data[:n], torch.ones(n, device=DEV), m, v, step, 0.1, (0.9, 0.99), 1e-8,
+                                             0.0, 1.0, norm=norm), lambda: f.data.mul_(0.5)):
+        write()
+        assert not all(f.packs.valid(e) for e in f.packs.entries.values())
+        new = conv(D.w0)
+        assert not torch.equal(old, new) and torch.equal(new, fresh())
+        assert torch.equal(conv(D.w0), new) and all(f.packs.valid(e) for e in f.packs.entries.values())
+        old = new
+    assert step._version and norm._version
+    f.grad.fill_(0.01)
+    opt.step()
+    assert all(f.packs.valid(e) for e in f.packs.entries.values())
+    assert not torch.equal(conv(D.w0), old) and torch.equal(conv(D.w0), fresh())
