@@ -80,7 +80,7 @@ class FusedAdamW:
         self.exp_avg = torch.zeros(self.flat.n_train, device=dev, dtype=torch.float32)
         self.exp_avg_sq = torch.zeros_like(self.exp_avg)
         self.step_count = torch.zeros(1, device=dev, dtype=torch.int32)
-        self.max_grad_norm = max_grad_norm
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
         self.grad_norm = torch.zeros((), device=dev, dtype=torch.float32)
 
     def zero_grad(self, set_to_none: bool = False):
@@ -104,8 +104,9 @@ class FusedAdamW:
     def step(self):
         f = self.flat
         if self.max_grad_norm is not None:
-            clipped_adamw_(f.data[:f.n_train], f.grad, self.exp_avg, self.exp_avg_sq, self.step_count, self.lr,
-                           self.betas, self.eps, self.weight_decay, self.max_grad_norm, norm=self.grad_norm)
+            clipped_adamw_(f.data[:f.n_train], f.grad, self.exp_avg, self.exp_avg_sq, self.step_count, float(self.lr),
+                           (float(self.betas[0]), float(self.betas[1])), float(self.eps), float(self.weight_decay),
+                           float(self.max_grad_norm), norm=self.grad_norm)
         else:
             check(LIB.ganamd_adamw(ptr(f.data), ptr(f.grad), ptr(self.exp_avg), ptr(self.exp_avg_sq), f.n_train,
                                    iptr(self.step_count), float(self.lr), float(self.betas[0]), float(self.betas[1]),

@@ -59,7 +59,7 @@ class Train(CheckpointMixin):
             raise ValueError(f"max_grad_norm {max_grad_norm}")
         self.optimizer_G, self.optimizer_D = self.make_optimizers()
         if max_grad_norm is not None:
-            self.optimizer_G.max_grad_norm = self.optimizer_D.max_grad_norm = max_grad_norm
+            self.optimizer_G.max_grad_norm = self.optimizer_D.max_grad_norm = float(max_grad_norm)
         # epoch bookkeeping of train/trainunits.py:25-28 (checkpoint names and resume)
         self.epoch, self.i = 0, 0
         try:

@@ -318,3 +318,29 @@ def test_plan_refuses_what_no_launch_holds(L, C, G, layout, dtype, op):
     assert lo == 65535 * 512 or threads(lo) * hi // lo >= 1 << 32
     for B in (2_100_000, 4_200_000, 33_000_000):
         assert threads(B) is None or threads(B) < 1 << 32
+
+
+def test_optimizer_numbers_of_any_kind(monkeypatch):
+    """lr, betas, eps, weight decay and the norm's limit as numpy scalars or 0-dim tensors, as the step
+    without a clip takes them: the native step is handed Python floats."""
+    import numpy as np
+    import gan_amd
+    from gan_amd import optim
+    seen = []
+    monkeypatch.setattr(optim, "clipped_adamw_", lambda *a, **k: seen.append(a))
+    one = lambda: torch.nn.Linear(2, 2)   # noqa: E731
+    tr = gan_amd.Train([], "cpu", 1, 4, one(), "g", one(), "d", rng=object(), max_grad_norm=torch.tensor(2.0))
+    for num in (np.float32, torch.tensor, np.float64, float):
+        opts = [optim.FusedAdamW(one(), lr=num(0.5), betas=(num(0.25), num(0.75)), eps=num(2.0 ** -20),
+                                 weight_decay=num(0.125), max_grad_norm=num(2.0)), tr.optimizer_D]
+        opts[1].lr, opts[1].betas, opts[1].eps, opts[1].weight_decay = num(0.5), (num(0.25), num(0.75)), num(2.0 ** -20), num(0.125)
+        for o in opts:
+            assert type(o.max_grad_norm) is float
+            o.step()
+            lr, betas, eps, wd, most = seen.pop()[5:]
+            got = (lr, *betas, eps, wd, most)
+            assert got == (0.5, 0.25, 0.75, 2.0 ** -20, 0.125, 2.0) and all(type(v) is float for v in got)
+            o.max_grad_norm = num(4.0)                   # set later
+            o.step()
+            assert seen.pop()[-1] == 4.0 and not seen
+            o.max_grad_norm = 2.0

@@ -1052,3 +1052,20 @@ def test_clipped_adamw_on_a_flat_buffer_counts_as_a_write(ops):
     opt.step()
     assert all(f.packs.valid(e) for e in f.packs.entries.values())
     assert not torch.equal(conv(D.w0), old) and torch.equal(conv(D.w0), fresh())
+
+
+def test_optimizer_step_with_numbers_of_any_kind(ops):
+    import numpy as np
+    from gan_amd.optim import FusedAdamW
+    got = []
+    for num in (float, np.float32, torch.tensor):
+        m = torch.nn.Linear(5, 3).to(DEV)
+        with torch.no_grad():
+            for p in m.parameters():
+                p.fill_(0.5)
+        o = FusedAdamW(m, lr=num(0.25), betas=(num(0.5), num(0.75)), eps=num(2.0 ** -20), weight_decay=num(0.125),
+                       max_grad_norm=num(0.5))
+        o.flat.grad.fill_(1.0)
+        o.step()
+        got.append(o.flat.data.clone())
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
