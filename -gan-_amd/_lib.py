@@ -189,6 +189,14 @@ class GanAmdError(RuntimeError):
     pass
 
 
+def _same_sources(host_hash):
+    """_host.so fills in libganamd.so's structs: one of other sources is refused (GANAMD_SO, a library
+    built for a comparison, is taken as it is)."""
+    if not os.environ.get("GANAMD_SO") and not LIB.ganamd_version().decode().endswith("src:" + host_hash):
+        raise ImportError(f"{_HERE}: libganamd.so ({LIB.ganamd_version().decode()}) and _host.so (src:{host_hash}) were "
+                          "built from different sources; build both with `python -c 'import __graft_entry__ as g; g.build()'`")
+
+
 def _load_host():
     """The module _host.so (csrc/host.cpp): autograd nodes and list reading of the operators whose
     host side is native.  It calls LIB's entry points, handed over by address."""
@@ -196,6 +204,7 @@ def _load_host():
         from . import _host
     except ImportError as e:
         raise ImportError(f"{_HERE}/_host.so: {e}; build it with `python -c 'import __graft_entry__ as g; g.build()'`") from e
+    _same_sources(getattr(_host, "SRC_HASH", "none"))
     _host.init(GanAmdError, {n: ctypes.cast(getattr(LIB, n), vp).value for n in _SIGS})
     return _host
 

@@ -642,4 +642,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&module); }
+// SRC_HASH: hash of the sources this module was compiled with (set by __graft_entry__.build()); the loader
+// compares it with libganamd.so's, whose structs this module fills in.
+#ifndef GANAMD_SRC_HASH
+#define GANAMD_SRC_HASH "unknown"
+#endif
+PyMODINIT_FUNC PyInit__host() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "SRC_HASH", GANAMD_SRC_HASH) < 0) Py_CLEAR(m);
+  return m;
+}

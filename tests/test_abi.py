@@ -285,3 +285,33 @@ def test_python_call_sites_match_signatures():
             if n is not None and n != want:
                 bad.append(f"{fn}:{node.lineno} {name}: {n} arguments, signature has {want}")
     assert not bad, bad
+
+
+def test_source_hash_covers_every_source(tmp_path, monkeypatch):
+    """A change to any file that either library is compiled from changes the hash."""
+    import shutil
+    import __graft_entry__ as g
+    shutil.copytree(os.path.join(g.PKG, "csrc"), tmp_path / "pkg" / "csrc")
+    shutil.copytree(os.path.join(g.REPO, "include"), tmp_path / "include")
+    monkeypatch.setattr(g, "PKG", str(tmp_path / "pkg"))
+    monkeypatch.setattr(g, "REPO", str(tmp_path))
+    seen = {g.source_hash()}
+    files = sorted((tmp_path / "pkg" / "csrc").iterdir()) + sorted((tmp_path / "include").iterdir())
+    assert any(f.name == "host.cpp" for f in files)
+    for f in files:
+        with open(f, "a") as o:
+            o.write("// changed")
+        h = g.source_hash()
+        assert h not in seen, f.name
+        seen.add(h)
+
+
+def test_host_module_is_of_the_same_sources(monkeypatch):
+    import __graft_entry__
+    from gan_amd import _lib
+    assert _lib.HOST.SRC_HASH == __graft_entry__.source_hash()
+    monkeypatch.delenv("GANAMD_SO", raising=False)
+    _lib._same_sources(_lib.HOST.SRC_HASH)
+    for other in ("0123456789abcdef", "none", "unknown"):
+        with pytest.raises(ImportError, match="different sources"):
+            _lib._same_sources(other)
