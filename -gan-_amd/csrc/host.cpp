@@ -600,6 +600,30 @@ PyObject* crosses(PyObject*, PyObject* o) {
   });
 }
 
+// Whether stream s is recording into a graph.  (The default stream cannot, and may not be asked while another does.)
+bool capturing(const c10::Stream& s) {
+  if (s.id() == 0) return false;
+  const auto type = c10::hip::getCurrentHIPStream(s.device_index()).unwrap().device_type();
+  const auto h = c10::hip::HIPStream::unpack3(s.id(), s.device_index(), type);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(h.stream(), &status) != hipSuccess) throw Refused("hipStreamIsCapturing failed");
+  return status != hipStreamCaptureStatusNone;
+}
+
+// apart(p): whether the backward node that is running and the accumulator of p's gradient are on different
+// streams that the engine could order, so that a gradient has to be handed to it (gan_amd.ops.flat_grad).
+// A node in a capture whose parameter's accumulator is outside it cannot be ordered with that at all: False.
+PyObject* apart(PyObject*, PyObject* o) {
+  return guarded("apart", [&]() -> PyObject* {
+    const auto node = torch::autograd::get_current_node();
+    const auto acc = torch::autograd::impl::try_get_grad_accumulator(tensor(o, "p"));
+    if (!node || !acc) Py_RETURN_FALSE;
+    const auto from = node->stream(), to = acc->stream();
+    if (!from || !to || *from == *to || (capturing(*from) && !capturing(*to))) Py_RETURN_FALSE;
+    Py_RETURN_TRUE;
+  });
+}
+
 // init(GanAmdError, {entry point: address})
 PyObject* init(PyObject*, PyObject* args) {
   PyObject *error = nullptr, *where = nullptr;
@@ -637,6 +661,7 @@ PyMethodDef methods[] = {
     {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(clip)), METH_FASTCALL, nullptr},
     {"clipped_adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(clipped_adamw)), METH_FASTCALL, nullptr},
     {"crosses", crosses, METH_O, nullptr},
+    {"apart", apart, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -412,14 +412,16 @@ def flat_grad(p):
     the Parameter a view ``p`` comes from): the backward then accumulates into it with its own
     kernel and returns None to autograd -- no per-parameter AccumulateGrad add launch (10k of them
     per generator step otherwise).  None when autograd has to handle it (create_graph backward,
-    parameters outside an optimizer's flat buffer, plain tensors)."""
+    parameters outside an optimizer's flat buffer, plain tensors; a parameter whose accumulator is on
+    another stream than the running node, used on two streams or held by an older graph: the engine
+    orders streams only along the gradients that it is handed)."""
     if p is None or torch.is_grad_enabled():
         return None
     root = p if p._base is None else p._base
     if not isinstance(root, torch.nn.Parameter) or getattr(root, "_gan_flat", None) is None:
         return None
     g = root.grad
-    if g is None or not g.is_contiguous() or g.numel() != p.numel():
+    if g is None or not g.is_contiguous() or g.numel() != p.numel() or _lib.HOST.apart(root):
         return None
     return g
 
