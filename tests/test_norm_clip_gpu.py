@@ -1069,3 +1069,52 @@ def test_optimizer_step_with_numbers_of_any_kind(ops):
         o.step()
         got.append(o.flat.data.clone())
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+@pytest.mark.parametrize("dtypes", [[F32], [BF16], [F16], [F32, BF16, F16]])
+@pytest.mark.parametrize("to", ["place", "same", "f32"])
+def test_clip_misaligned(ops, dtypes, to):
+    """Gradients and outputs that start one, two and three elements into their buffers, each output
+    elsewhere than its gradient; what surrounds the outputs stays."""
+    sizes = [1, 2, 9, 255, 4096, 8191, 30_001]
+    ts = grads(sizes, dtypes, 8)
+    n = norm64(ts)
+    c = 0.37 * n / (n + 1e-6)
+
+    def off(t, k, dt=None):
+        room = torch.full((t.numel() + 8,), 7.0, dtype=dt or t.dtype, device=DEV)
+        view = room[k:k + t.numel()]
+        if dt is None:
+            view.copy_(t)
+        return room, view
+
+    src = [off(t, 1 + i % 3) for i, t in enumerate(ts)]
+    dst = src if to == "place" else [off(t, 1 + (i + 1) % 3, t.dtype if to == "same" else F32) for i, t in enumerate(ts)]
+    got = ops.clip_grad_norm_([v for _, v in src], 0.37 * n, out=None if to == "place" else [v for _, v in dst])
+    assert abs(float(got) - n) <= 2.0 ** -23 * n
+    for t, (room, o), (_, s) in zip(ts, dst, src):
+        want = t.double() * c
+        lim = want.abs() * (2 * 2.0 ** -24 * 1.01 + HALF[o.dtype]) + TINY[o.dtype]
+        assert bool(((o.double() - want).abs() <= lim).all())
+        at = o.storage_offset()
+        assert bool((room[:at] == 7).all()) and bool((room[at + t.numel():] == 7).all())
+        assert to == "place" or torch.equal(s, t)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_clip_permuted_in_place(ops, dtype):
+    """Tensors of other memory orders, scaled in place and into outputs of their own strides."""
+    g = torch.Generator().manual_seed(9)
+    make_ = lambda *s: torch.randn(*s, generator=g).to(dtype).to(DEV)   # noqa: E731
+    for out in (False, True):
+        ts = [make_(6, 5, 4, 3).to(memory_format=torch.channels_last), make_(31, 7).t(), make_(9, 8, 7).permute(2, 0, 1),
+              make_(33, 1, 5).transpose(0, 1)]
+        ref = [t.double() for t in ts]
+        n = norm64(ts)
+        c = 0.5 * n / (n + 1e-6)
+        dst = [torch.empty_like(t) for t in ts] if out else ts
+        ops.clip_grad_norm_(ts, 0.5 * n, out=dst if out else None)
+        for o, r, t in zip(dst, ref, ts):
+            assert o.stride() == t.stride()
+            lim = (r * c).abs() * (2 * 2.0 ** -24 * 1.01 + HALF[dtype]) + TINY[dtype]
+            assert bool(((o.double() - r * c).abs() <= lim).all())
