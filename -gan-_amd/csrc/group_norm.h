@@ -17,8 +17,12 @@
 //
 // Statistics are summed and kept in 64 bits: the sign of z selects the branch of a kinked
 // activation, and at fp32 accuracy a handful of values per 10^7 fall on the wrong side, each an
-// error of the size of the gradient.  The test itself is one fp32 comparison of x with the
-// channel's threshold (the smallest float whose z is positive), exact for every x.
+// error of the size of the gradient.  What is summed are the differences from a pivot, the group's first
+// value: |pivot - mean| is at most sqrt(N) standard deviations, so what cancels between their mean
+// square and their squared mean is at most N variances, in 64 bits, wherever the mean lies (sums of x
+// and x^2 put the gradient of a group of one value 3e5 repeated off by 9 %).  The test itself is one
+// fp32 comparison of x with the channel's threshold (the smallest float whose z is positive), exact
+// for every x.
 //
 // What bounds them: memory.  Two forms:
 //  * resident: one block holds all of a group's (rows: a tile of whole groups') values in
@@ -50,7 +54,8 @@ struct Args {
   float cslope;                                 // constant slope where slope is null
   float eps;
   long L, B;                                    // positions, samples
-  int C, G, Cg, pdt;
+  int C, G, Cg, pdt, xdt;
+  long pb, pc;                                  // elements from a sample / a channel to the next
   int TX, P;                                    // threads across the channels (rows) / planes per block; positions in flight
   int CT, nct;                                  // channels per tile, tiles
   int S;                                        // chunks of a sample's positions
@@ -97,19 +102,20 @@ struct Vec {
   uint32_t w[N];
   __device__ __forceinline__ float get(int j) const;
   __device__ __forceinline__ void put(const float (&f)[V]);
-  // elements j < n become zero
-  __device__ __forceinline__ void zero_front(int n) {
+  // elements j < n become the value of these bits
+  __device__ __forceinline__ void fill_front(int n, uint32_t v) {
     if (n <= 0) return;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (PER == 1) {
-        if (i < n) w[i] = 0;
+        if (i < n) w[i] = v;
       } else {
         const int k = n - 2 * i;
-        w[i] = k >= 2 ? 0u : k == 1 ? w[i] & 0xffff0000u : w[i];
+        w[i] = k >= 2 ? v | v << 16 : k == 1 ? (w[i] & 0xffff0000u) | v : w[i];
       }
     }
   }
+  __device__ __forceinline__ void zero_front(int n) { fill_front(n, 0); }
   // the compiler may not carry anything derived from these words past here
   __device__ __forceinline__ void pin() {
 #pragma unroll
@@ -186,10 +192,15 @@ __device__ __forceinline__ float loadp(const void* p, int dt, long i) {
   return up(static_cast<const f16*>(p)[i]);
 }
 
+// The pivot of channel c's group in sample b: its first value.
+__device__ __forceinline__ float pivot(const Args& a, long b, int c) {
+  return loadp(a.x, a.xdt, b * a.pb + (long)(c / a.Cg * a.Cg) * a.pc);
+}
+
 // ------------------------------------------------------------------ which elements a thread owns
 // rows (channels last): V consecutive channels, every P-th position.  planes (channel rows): one
 // channel, every P-th vector of V positions.  The last vector of a row / plane is moved back to end
-// with it; its first `skip` elements belong to its neighbour and count as zero here.
+// with it; its first `skip` elements belong to its neighbour and add nothing to the sums here.
 template <bool ROWS, int V>
 struct Map {
   long base, step;     // element offset of position 0, of one position
@@ -321,7 +332,8 @@ __device__ __forceinline__ float act_d1(const Chan<MODE, ACT>& c, float x, float
 }
 
 // ------------------------------------------------------------------ sums over positions
-// FWD sums in double (x, x^2); the others in fp32 over a thread's own positions.
+// FWD sums in double (x - pivot and its square; ch.mf holds the pivot); the others in fp32 over a
+// thread's own positions.
 //   BWD: g, g d (, gy z [z<=0]).   DBL: v, v d, g, g d, g v, then
 //   SILU: k, k d, k d^2, k v, k v d with k = gy a''; SLOPE: s, s d, s v with s = gy [z <= 0]
 template <int MODE, int ACT>
@@ -342,7 +354,7 @@ __device__ __forceinline__ void accumulate(A (&acc)[K][NC], const Chan<MODE, ACT
     const int c = ROWS ? j : 0;
     const float xf = x.get(j);
     if constexpr (MODE == FWD) {
-      const double xd = (double)xf;
+      const double xd = (double)xf - (double)ch[c].mf;
       acc[0][c] += xd;
       acc[1][c] = fma(xd, xd, acc[1][c]);
     } else {
@@ -642,6 +654,30 @@ __device__ __forceinline__ void apply(const Lin<MODE, ACT> (&ln)[NC], const Vec<
 }
 
 // ------------------------------------------------------------------ shared by the kernels
+// The pivots of a thread's channels (FWD's only channel constants): asked for before its data, of the
+// first two groups that the channels lie in and without a branch, so that nothing waits for them
+// before the data is on its way; put to use after that (narrower groups: read one by one then).
+template <int ACT, bool ROWS, class T, int V, int NC>
+struct Pivots {
+  const T* x;
+  T p0, p1;
+  int g, rest;                             // the first group's first channel, channels left in it
+  __device__ __forceinline__ Pivots(const Args& a, const Map<ROWS, V>& m, long b) {
+    x = static_cast<const T*>(a.x) + b * a.pb;
+    g = m.ch / a.Cg * a.Cg;
+    rest = a.Cg - (m.ch - g);
+    p0 = x[g * a.pc];
+    if (NC > 1) p1 = x[min(g + a.Cg, a.C - a.Cg) * a.pc];
+  }
+  __device__ __forceinline__ void get(const Args& a, Chan<FWD, ACT> (&ch)[NC]) const {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) ch[j].mf = NC == 1 || j < rest ? up(p0) : up(p1);
+    if (NC > 1 && a.Cg + 1 < NC)
+#pragma unroll
+      for (int j = 1; j < NC; ++j) ch[j].mf = up(x[(g + (a.Cg - rest + j) / a.Cg * a.Cg) * a.pc]);
+  }
+};
+
 // A tile's channel constants for the sums (BWD, DBL): made in `tab`, read by every thread.
 template <int MODE, int ACT, bool ROWS, int V, int NC>
 __device__ __forceinline__ void load_chan(const Args& a, const Map<ROWS, V>& m, long b, int c0, float* tab,
@@ -682,8 +718,8 @@ __device__ __forceinline__ void load_lin(const Args& a, const Map<ROWS, V>& m, l
 }
 
 // Groups c0 / Cg .. of sample b from their channels' sums chan[k * stride + c], W lanes each (the
-// channels of a group, at most a wave): statistics or coefficients to gco[8 a group], a sample's
-// terms of the parameter gradients to par.
+// channels of a group, at most a wave): statistics or coefficients to gco[8 a group] (FWD: which holds the
+// pivots in field 7), a sample's terms of the parameter gradients to par.
 template <int MODE, int ACT, class A>
 __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int ng, const A* chan, long stride,
                                               double* gco, bool tell) {
@@ -703,7 +739,7 @@ __device__ __forceinline__ void finish_groups(const Args& a, long b, int c0, int
       }
       s = lanes_sum(s, W);
       q = lanes_sum(q, W);
-      const double mean = s * invN, var = fmax(q * invN - mean * mean, 0.0);
+      const double md = s * invN, mean = co[7] + md, var = fmax(q * invN - md * md, 0.0);
       const double nan = s - s + (q - q);            // fmax drops a NaN: put it back
       const double r = 1.0 / sqrt(var + nan + (double)a.eps);
       if (lane == 0) {
@@ -780,6 +816,10 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
   const T* pg = static_cast<const T*>(a.gy);
   const T* pv = static_cast<const T*>(a.v);
 
+  const int c0 = tile * a.CT, g0 = c0 / a.Cg, ng = min(gt, a.G - g0);
+  Chan<MODE, ACT> ch[NC];
+  const Pivots<ACT, ROWS, T, V, NC> piv(a, m, b);
+  const T mine = static_cast<const T*>(a.x)[b * a.pb + (c0 + min((int)threadIdx.x, ng - 1) * a.Cg) * a.pc];
   Vec<T, V> x[RMAX], gy[MODE >= BWD ? RMAX : 1], v[MODE == DBL ? RMAX : 1];
 #pragma unroll
   for (int k = 0; k < RMAX; ++k) {
@@ -791,12 +831,15 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
       if constexpr (MODE >= BWD) gy[k] = load<T, V>(pg + at);
       if constexpr (MODE == DBL) v[k] = load<T, V>(pv + at);
     }
-    if (MODE == FWD || skip == V) x[k].zero_front(skip);
+    if (MODE != FWD && skip == V) x[k].zero_front(skip);
     if constexpr (MODE >= BWD) gy[k].zero_front(skip);
     if constexpr (MODE == DBL) v[k].zero_front(skip);
   }
-  const int c0 = tile * a.CT, g0 = c0 / a.Cg, ng = min(gt, a.G - g0);
-  Chan<MODE, ACT> ch[NC];
+  if constexpr (MODE == FWD) {
+    if ((int)threadIdx.x < ng) gco[8 * threadIdx.x + 7] = (double)up(mine);
+    for (int g = threadIdx.x + blockDim.x; g < ng; g += blockDim.x) gco[8 * g + 7] = (double)pivot(a, b, c0 + g * a.Cg);
+    piv.get(a, ch);
+  }
   load_chan<MODE, ACT, ROWS, V, NC>(a, m, b, c0, tab, ch);
   A acc[K][NC];
 #pragma unroll
@@ -804,9 +847,20 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < NC; ++j) acc[k][j] = 0;
 #pragma unroll
-  for (int k = 0; k < RMAX; ++k)
-    if (m.active && (k == 0 || k * a.P < m.npos))
-      accumulate<MODE, ACT, ROWS, T, V, NC>(acc, ch, x[k], gy[MODE >= BWD ? k : 0], v[MODE == DBL ? k : 0]);
+  for (int k = 0; k < RMAX; ++k) {
+    if constexpr (MODE == FWD) {
+      const int i = m.p + k * a.P;
+      if (!m.active || i >= m.npos) continue;
+      if (!ROWS && a.L % V) {              // (rows: the fold leaves a moved-back front out)
+        int skip;
+        m.at(i, skip);
+        x[k].fill_front(skip, bits(down<T>(ch[0].mf)));
+      }
+    } else if (!m.active || (k > 0 && k * a.P >= m.npos)) {
+      continue;
+    }
+    accumulate<MODE, ACT, ROWS, T, V, NC>(acc, ch, x[k], gy[MODE >= BWD ? k : 0], v[MODE == DBL ? k : 0]);
+  }
 #pragma unroll
   for (int k = 0; k < RMAX; ++k) {
     x[k].pin();
@@ -920,16 +974,20 @@ __global__ __launch_bounds__(kNT) void sums_kernel(Args a) {
   const int c0 = tile * a.CT, wid = min(a.CT, a.C - c0);
   const int hi = (int)min((long)m.npos, (long)(s + 1) * a.per);
   Chan<MODE, ACT> ch[NC];
+  const Pivots<ACT, ROWS, T, V, NC> piv(a, m, b);
   A acc[K][NC];
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int j = 0; j < NC; ++j) acc[k][j] = 0;
   stream<MODE, ROWS, T, V, U>(
-      a, m, s * a.per, hi, [&] { load_chan<MODE, ACT, ROWS, V, NC>(a, m, b, c0, tab, ch); },
+      a, m, s * a.per, hi, [&] {
+        if constexpr (MODE == FWD) piv.get(a, ch);
+        load_chan<MODE, ACT, ROWS, V, NC>(a, m, b, c0, tab, ch);
+      },
       [&](long, int skip, Vec<T, V>& x, Vec<T, V>& gy, Vec<T, V>& v) {
         if constexpr (!ROWS) {                 // (rows: the fold leaves a moved-back front out)
-          if (MODE == FWD) x.zero_front(skip);
+          if (MODE == FWD) x.fill_front(skip, bits(down<T>(ch[0].mf)));
           if constexpr (MODE >= BWD) gy.zero_front(skip);
           if constexpr (MODE == DBL) v.zero_front(skip);
         }
@@ -963,8 +1021,13 @@ __global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) 
   constexpr int K = Sums<MODE, ACT>::K;
   const int nb = (a.G + gpb - 1) / gpb, g0 = blockIdx.x % nb * gpb, bi = blockIdx.x / nb;
   const long b = bi;
+  extern __shared__ __align__(16) double gco[];      // (FWD)
   const int ng = min(gpb, a.G - g0), nc = ng * a.Cg, pairs = K * nc, ns = (a.S + sstep - 1) / sstep;
   A* part = reinterpret_cast<A*>(a.part) + (long)bi * a.S * K * a.C + g0 * a.Cg;
+  if (MODE == FWD) {
+    for (int i = threadIdx.x; i < ng; i += 256) gco[8 * i + 7] = (double)pivot(a, b, (g0 + i) * a.Cg);
+    if (ns <= 1) __syncthreads();
+  }
   if (ns > 1) {
     int sw = 1;                                       // lanes that share a channel's chunks
     while (sw * 2 * pairs <= 256 && sw * 2 <= ns && sw < 64) sw *= 2;
@@ -984,7 +1047,6 @@ __global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) 
     __syncthreads();
   }
   // (FWD writes the statistics; the coefficients have their own place)
-  extern __shared__ __align__(16) double gco[];
   finish_groups<MODE, ACT>(a, b, g0 * a.Cg, ng, part, (long)a.C, MODE == FWD ? gco : a.coef + 8 * (b * a.G + g0),
                            true);
 }
@@ -1010,6 +1072,8 @@ __global__ __launch_bounds__(kNT) void apply_kernel(Args a, int fold_S) {
           double* gco = reinterpret_cast<double*>(lds);
           A* chan = reinterpret_cast<A*>(gco + 8L * a.G);            // [K][C]; then the coefficients
           const A* part = reinterpret_cast<const A*>(a.part) + b * fold_S * K * a.C;
+          if (MODE == FWD)
+            for (int g = threadIdx.x; g < a.G; g += blockDim.x) gco[8L * g + 7] = (double)pivot(a, b, g * a.Cg);
           for (int i = threadIdx.x; i < K * a.C; i += blockDim.x) {
             double t = 0;
 #pragma unroll 4

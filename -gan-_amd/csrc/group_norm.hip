@@ -57,6 +57,7 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   // of 32x32: forward 13.4 us against 16.7 with the widest blocks, backward 23.9 against 25.9).
   const long few = mode == gn::DBL ? 4 : 8;
   a.L = L; a.B = B; a.C = C; a.G = G; a.Cg = Cg; a.eps = d->eps; a.pdt = d->param_dtype;
+  a.xdt = d->dtype; a.pb = p.rows ? L * C : L; a.pc = p.rows ? 1 : B * L;
   a.cslope = d->act == GANAMD_NORM_LEAKY ? d->slope : 1.f;
   // A call whose tensors are well beyond the 256 MB of the last-level cache: its outputs are stored past
   // the caches (forward and a copy of its output, 256 maps of 64x64x96 in bf16: 190 us against 212;

@@ -1118,3 +1118,21 @@ def test_clip_permuted_in_place(ops, dtype):
             assert o.stride() == t.stride()
             lim = (r * c).abs() * (2 * 2.0 ** -24 * 1.01 + HALF[dtype]) + TINY[dtype]
             assert bool(((o.double() - r * c).abs() <= lim).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("value", [1e4, -3e5, 1e6, 1e8])
+@pytest.mark.parametrize("shape,G,layout", [((2, 9, 9, 12), 2, "nhwc"), ((1, 3000, 8), 2, "nhwc"), ((2, 40, 37, 12), 3, "nhwc"),
+                                            ((12, 2, 9, 9), 2, "cnhw"), ((4, 1, 40000), 2, "cnhw")])
+def test_group_norm_large_constant_group(ops, shape, G, layout, dtype, value):
+    """A group of one large value repeated has variance 0, not the rounding of its square."""
+    t = make(shape, layout, "silu", dtype, 8)
+    t["x"].fill_(value)
+    check_all(ops, t, G, "silu", layout)
+
+
+@pytest.mark.parametrize("shape,G,layout", [((2, 16, 16, 12), 3, "nhwc"), ((1, 3000, 8), 2, "nhwc"), ((2, 40, 37, 12), 3, "nhwc"),
+                                            ((12, 2, 16, 16), 3, "cnhw"), ((4, 1, 40000), 2, "cnhw")])
+def test_group_norm_very_far_mean(ops, shape, G, layout):
+    """Values of spread 1 around 3e6, where fp32 steps by a quarter."""
+    check_all(ops, make(shape, layout, "silu", F32, 7, scale=1.0, shift=3e6), G, "silu", layout)
