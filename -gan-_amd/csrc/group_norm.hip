@@ -56,6 +56,14 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   // this many vectors of an input: several blocks a CU overlap their phases (64 samples of 128 rows
   // of 32x32: forward 13.4 us against 16.7 with the widest blocks, backward 23.9 against 25.9).
   const long few = mode == gn::DBL ? 4 : 8;
+  // A block of the resident form that holds so few values beats the split form's launches however few the
+  // blocks are (one fp32 sample, resident against split: forward of 64 channels of 16x16, 8 K values a block,
+  // 6.3 us against 9.6, of 32x32, 32 K, 9.5 against 10.1; backward 11.1 against 14.0, of 16x32, 16 K, 12.0 against
+  // 13.6).  A larger one takes longer than they do (forward of 4 bf16 samples of 32x32x128, 64 K, 16.2 against
+  // 13.4; backward of one sample of 64 channels of 32x32 17.2 against 13.5) until there are many blocks
+  // (that one, 96 blocks: forward 11.7 against 14.9, backward 23.1 against 21.1; 192: 13.8 against 19.4, 25.1
+  // against 32.3).
+  const long small = mode == gn::FWD ? 32 << 10 : 16 << 10, many = 96;
   a.L = L; a.B = B; a.C = C; a.G = G; a.Cg = Cg; a.eps = d->eps; a.pdt = d->param_dtype;
   a.xdt = d->dtype; a.pb = p.rows ? L * C : L; a.pc = p.rows ? 1 : B * L;
   a.cslope = d->act == GANAMD_NORM_LEAKY ? d->slope : 1.f;
@@ -79,7 +87,7 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     if (TX <= most) {
       const long P = std::min(most / TX, std::max(up_to(L, few), std::min(L, 256 / TX)));
       const long R = up_to(L, P), nct = up_to(G, gt);
-      if (R <= rcap && (R <= 2 || B * nct >= 96)) {
+      if (R <= rcap && (CT * L <= small || B * nct >= many)) {
         p.resident = true;
         a.TX = (int)TX; a.P = (int)P; a.CT = (int)CT; a.nct = (int)nct; p.rmax = (int)R;
         p.nt = (int)up_to(TX * P, 64) * 64;
@@ -87,10 +95,15 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
     }
   } else if (Cg <= most) {
     long P = std::min(pow2_at_least(nv), pow2_at_least(most / Cg + 1) / 2), gt = 1;
-    while (gt < G && (gt + 1) * Cg * P <= 256 && B * up_to(G, gt + 1) >= 512) ++gt;
+    // Small planes: several groups a block, up to 512 threads while two blocks a CU are left (forward of 1024
+    // samples of 64 planes of 4x4, groups of 2: 6.1 us, one group a block 24; 256 samples of 128 planes of 8x8,
+    // groups of 4: 6.9 us, up to 256 threads 7.9; 512 bf16 samples of 32 planes of 8x8: 5.2 us, with four
+    // blocks a CU left 5.9, with one 5.3).
+    while (gt < G && (gt + 1) * Cg * P <= 512 && B * up_to(G, gt + 1) >= 512) ++gt;
+    gt = up_to(G, up_to(G, gt));           // (as many blocks, evenly filled)
     while (P > 1 && up_to(nv, P / 2) <= few && gt * Cg * P > 256) P /= 2;
     const long R = up_to(nv, P), nct = up_to(G, gt);
-    if (R <= rcap && (R <= 2 || B * nct >= 96)) {
+    if (R <= rcap && (gt * Cg * L <= small || B * nct >= many)) {
       p.resident = true;
       a.TX = (int)(gt * Cg); a.P = (int)P; a.CT = (int)(gt * Cg); a.nct = (int)nct; p.rmax = (int)R;
       p.nt = (int)up_to(a.TX * P, 64) * 64;
