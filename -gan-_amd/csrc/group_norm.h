@@ -192,9 +192,16 @@ __device__ __forceinline__ float loadp(const void* p, int dt, long i) {
   return up(static_cast<const f16*>(p)[i]);
 }
 
-// The pivot of channel c's group in sample b: its first value.
-__device__ __forceinline__ float pivot(const Args& a, long b, int c) {
-  return loadp(a.x, a.xdt, b * a.pb + (long)(c / a.Cg * a.Cg) * a.pc);
+// The pivot of the group that starts with channel c, in sample b: its first value.
+__device__ __forceinline__ float pivot(const Args& a, long b, int c) { return loadp(a.x, a.xdt, b * a.pb + c * a.pc); }
+// The same as it is stored, so that nothing waits for the load before the value is put to use.
+__device__ __forceinline__ uint32_t pivot_bits(const Args& a, long b, int c) {
+  const long i = b * a.pb + c * a.pc;
+  return a.xdt == GANAMD_F32 ? static_cast<const uint32_t*>(a.x)[i] : static_cast<const uint16_t*>(a.x)[i];
+}
+__device__ __forceinline__ float of_bits(const Args& a, uint32_t v) {
+  return a.xdt == GANAMD_F32 ? __uint_as_float(v) : a.xdt == GANAMD_BF16 ? up(bf16{(uint16_t)v})
+       : (float)__builtin_bit_cast(_Float16, (uint16_t)v);
 }
 
 // ------------------------------------------------------------------ which elements a thread owns
@@ -1024,10 +1031,7 @@ __global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) 
   extern __shared__ __align__(16) double gco[];      // (FWD)
   const int ng = min(gpb, a.G - g0), nc = ng * a.Cg, pairs = K * nc, ns = (a.S + sstep - 1) / sstep;
   A* part = reinterpret_cast<A*>(a.part) + (long)bi * a.S * K * a.C + g0 * a.Cg;
-  if (MODE == FWD) {
-    for (int i = threadIdx.x; i < ng; i += 256) gco[8 * i + 7] = (double)pivot(a, b, (g0 + i) * a.Cg);
-    if (ns <= 1) __syncthreads();
-  }
+  const uint32_t mine = MODE == FWD ? pivot_bits(a, b, (g0 + min((int)threadIdx.x, ng - 1)) * a.Cg) : 0;
   if (ns > 1) {
     int sw = 1;                                       // lanes that share a channel's chunks
     while (sw * 2 * pairs <= 256 && sw * 2 <= ns && sw < 64) sw *= 2;
@@ -1044,8 +1048,9 @@ __global__ __launch_bounds__(256) void group_kernel(Args a, int gpb, int sstep) 
       t = lanes_sum(t, sw);
       if (q == 0 && i < pairs) *p = (A)t;
     }
-    __syncthreads();
   }
+  if (MODE == FWD && (int)threadIdx.x < ng) gco[8 * threadIdx.x + 7] = (double)of_bits(a, mine);   // (gpb <= 128)
+  if (MODE == FWD || ns > 1) __syncthreads();
   // (FWD writes the statistics; the coefficients have their own place)
   finish_groups<MODE, ACT>(a, b, g0 * a.Cg, ng, part, (long)a.C, MODE == FWD ? gco : a.coef + 8 * (b * a.G + g0),
                            true);
@@ -1072,13 +1077,16 @@ __global__ __launch_bounds__(kNT) void apply_kernel(Args a, int fold_S) {
           double* gco = reinterpret_cast<double*>(lds);
           A* chan = reinterpret_cast<A*>(gco + 8L * a.G);            // [K][C]; then the coefficients
           const A* part = reinterpret_cast<const A*>(a.part) + b * fold_S * K * a.C;
-          if (MODE == FWD)
-            for (int g = threadIdx.x; g < a.G; g += blockDim.x) gco[8L * g + 7] = (double)pivot(a, b, g * a.Cg);
+          const T mine = static_cast<const T*>(a.x)[b * a.pb + min((int)threadIdx.x, a.G - 1) * a.Cg * a.pc];
           for (int i = threadIdx.x; i < K * a.C; i += blockDim.x) {
             double t = 0;
 #pragma unroll 4
             for (int k = 0; k < fold_S; ++k) t += (double)part[(long)k * K * a.C + i];
             chan[i] = (A)t;
+          }
+          if (MODE == FWD) {
+            if ((int)threadIdx.x < a.G) gco[8 * threadIdx.x + 7] = (double)up(mine);
+            for (int g = threadIdx.x + blockDim.x; g < a.G; g += blockDim.x) gco[8 * g + 7] = (double)pivot(a, b, g * a.Cg);
           }
           __syncthreads();
           finish_groups<MODE, ACT>(a, b, 0, a.G, chan, (long)a.C, gco, s == 0);
