@@ -805,7 +805,8 @@ __device__ __forceinline__ void write(const Args& a, const Lin<MODE, ACT> (&ln)[
 // Block (tile of whole groups, sample): RMAX vectors a thread, held between sums and result, so each
 // input is read once.  What is left above a copy's time is that a block's phases follow each other
 // (load, fold, coefficients, store): 64 samples of 48 channel rows of 64x64 in fp32, forward 20 us
-// (5.0 TB/s), backward 35 (4.3); of 128 rows of 32x32 forward 16, backward 20, double backward 36 (4.7).
+// (5.0 TB/s), backward 35 (4.3); of 128 rows of 32x32 forward 16, backward 20, double backward 36 (4.7);
+// in bf16 16, 22 and 12, 14, 22 (half the bytes: the phases weigh more).
 template <int MODE, int ACT, bool ROWS, class T, int V, int RMAX, int NTMAX>
 __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
   typedef typename AccT<MODE>::type A;
@@ -898,7 +899,7 @@ __global__ __launch_bounds__(NTMAX) void resident_kernel(Args a) {
 // For groups that no block can hold (channels last, a group's values lie a few channels wide over all
 // positions: reading one alone would fetch every line for each group).  The second pass reads the
 // inputs again: 64 maps of 64x64x96 in bf16, forward 15 us of sums and 20 of the elementwise pass; 256
-// of them 42 and 62 (4.8 and 6.5 TB/s), backward 68 and 108 (5.9 and 5.6).  Neither waits on the
+// of them 43 and 62 (4.7 and 6.5 TB/s), backward 68 and 108 (5.9 and 5.6).  Neither waits on the
 // vector units (a leaky slope takes the same time as SiLU).
 constexpr int kNT = 512;
 

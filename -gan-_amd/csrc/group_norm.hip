@@ -54,7 +54,8 @@ bool make_plan(const ganamd_norm_desc* d, int mode, Full& f) {
   const int rcap = gn::resident_vectors(mode, p.rows), most = gn::resident_threads(mode, p.rows);
   // Resident blocks are made smaller, down to 256 threads, as long as a thread then holds no more than
   // this many vectors of an input: several blocks a CU overlap their phases (64 samples of 128 rows
-  // of 32x32: forward 13.4 us against 16.7 with the widest blocks, backward 23.9 against 25.9).
+  // of 32x32, calls back to back: forward 13.4 us against 16.7 with the widest blocks, backward 23.9 against
+  // 25.9).
   const long few = mode == gn::DBL ? 4 : 8;
   // A block of the resident form that holds so few values beats the split form's launches however few the
   // blocks are (one fp32 sample, resident against split: forward of 64 channels of 16x16, 8 K values a block,
