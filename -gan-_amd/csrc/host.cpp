@@ -100,6 +100,11 @@ Tensor norm_forward(const ganamd_norm_desc& d, const Tensor& x, const Tensor& w,
   return y;
 }
 
+// Whether p has hooks that autograd runs on its gradient: they see only gradients that the engine is handed.
+bool hooked(const Tensor& p) {
+  return !torch::autograd::impl::hooks(p).empty() || torch::autograd::impl::post_acc_grad_hooks(p) != nullptr;
+}
+
 // Where the gradients of w, b and slope go: new tensors; or, where every wanted one is of a
 // parameter in a flat buffer and this is a first-order backward, the buffer's views themselves
 // (added to; the engine then gets none).  The engine orders streams along the gradients that it is
@@ -127,7 +132,7 @@ Targets targets(const Tensor* par, const bool* want, int64_t flat) {
     // a gradient that autograd.grad was asked for is returned, not added
     const auto node = torch::autograd::impl::try_get_grad_accumulator(par[i]);
     const auto* info = torch::autograd::get_current_graph_task_exec_info();
-    all = all && node && node->stream() == self->stream();
+    all = all && node && node->stream() == self->stream() && !hooked(par[i]);
     if (node && info) {
       const auto it = info->find(node.get());
       if (it != info->end() && it->second.captures_) all = false;
@@ -610,14 +615,17 @@ bool capturing(const c10::Stream& s) {
   return status != hipStreamCaptureStatusNone;
 }
 
-// apart(p): whether the backward node that is running and the accumulator of p's gradient are on different
-// streams that the engine could order, so that a gradient has to be handed to it (gan_amd.ops.flat_grad).
+// apart(p): whether p's gradient has to be handed to the engine (gan_amd.ops.flat_grad): p has hooks, or the
+// backward node that is running and the accumulator of p's gradient are on different streams that the engine
+// could order.
 // A node in a capture whose parameter's accumulator is outside it cannot be ordered with that at all: False.
 PyObject* apart(PyObject*, PyObject* o) {
   return guarded("apart", [&]() -> PyObject* {
     const auto node = torch::autograd::get_current_node();
-    const auto acc = torch::autograd::impl::try_get_grad_accumulator(tensor(o, "p"));
+    const Tensor& p = tensor(o, "p");
+    const auto acc = torch::autograd::impl::try_get_grad_accumulator(p);
     if (!node || !acc) Py_RETURN_FALSE;
+    if (hooked(p)) Py_RETURN_TRUE;
     const auto from = node->stream(), to = acc->stream();
     if (!from || !to || *from == *to || (capturing(*from) && !capturing(*to))) Py_RETURN_FALSE;
     Py_RETURN_TRUE;

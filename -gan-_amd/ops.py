@@ -412,9 +412,9 @@ def flat_grad(p):
     the Parameter a view ``p`` comes from): the backward then accumulates into it with its own
     kernel and returns None to autograd -- no per-parameter AccumulateGrad add launch (10k of them
     per generator step otherwise).  None when autograd has to handle it (create_graph backward,
-    parameters outside an optimizer's flat buffer, plain tensors; a parameter whose accumulator is on
-    another stream than the running node, used on two streams or held by an older graph: the engine
-    orders streams only along the gradients that it is handed)."""
+    parameters outside an optimizer's flat buffer, plain tensors; a parameter with gradient hooks, or
+    whose accumulator is on another stream than the running node, used on two streams or held by an
+    older graph: hooks see, and the engine orders streams along, only gradients that it is handed)."""
     if p is None or torch.is_grad_enabled():
         return None
     root = p if p._base is None else p._base
@@ -1527,8 +1527,8 @@ def group_norm_act(x, groups: int, weight=None, bias=None, act: str = "none", sl
     None (ones / zeros).  ``act``: ``"none"``, ``"silu"``, ``"leaky"`` (``slope``: a number; 0 is a
     ReLU), ``"prelu"`` (``slope``: ``[C]``, with a gradient).  Parameters are all float32 or all of
     x's type, as are their gradients; the arithmetic is float32, statistics float64.  Gradients of
-    parameters in an optimizer's flat buffer are added there by the kernel, where the backward runs on
-    the stream that the parameters' accumulators belong to (else autograd adds them).
+    parameters in an optimizer's flat buffer are added there by the kernel, where they have no hooks and
+    the backward runs on the stream that their accumulators belong to (else autograd adds them).
     A non-contiguous ``x`` is copied first; an empty one gives an empty result.  Forward-mode
     derivatives are refused.  A backward under
     graph capture whose inputs an eager result on the default stream still holds is refused
@@ -1558,7 +1558,7 @@ def grad_norm(tensors, norm_type: float = 2.0):
     """The norm of all ``tensors`` together as a 0-dim float32 tensor on their device (no host
     synchronisation): the root of the sum of all squares, summed in float64, or with ``norm_type``
     infinity the largest magnitude.  Tensors of any number, size (empty ones included) and of mixed
-    types; densely stored."""
+    types; densely stored.  Not differentiable (``no_grad``), as torch's."""
     kind = _norm_kind("grad_norm", norm_type)
     ts = _as_list(tensors)
     return _lib.HOST.grad_norm(ts, kind) if ts else torch.zeros((), device="cuda")

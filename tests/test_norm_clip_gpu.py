@@ -1136,3 +1136,31 @@ def test_group_norm_large_constant_group(ops, shape, G, layout, dtype, value):
 def test_group_norm_very_far_mean(ops, shape, G, layout):
     """Values of spread 1 around 3e6, where fp32 steps by a quarter."""
     check_all(ops, make(shape, layout, "silu", F32, 7, scale=1.0, shift=3e6), G, "silu", layout)
+
+
+@pytest.mark.parametrize("order", [1, 2])
+def test_group_norm_flat_gradients_with_hooks(ops, order):
+    """Gradient hooks of parameters in the flat buffer run, and what they return is what arrives there."""
+    D, t, pars, call, want = flat_case(ops, 38)
+
+    def back():
+        D._flat.grad.zero_()
+        x = t["x"].clone().requires_grad_()
+        if order == 1:
+            call(x).backward(t["gy"])
+        else:
+            (gx,) = torch.autograd.grad(call(x), x, t["gy"], create_graph=True)
+            gx.backward(t["v"], inputs=list(pars))
+        return [p.grad.clone() for p in pars]
+
+    plain = back()
+    if order == 1:
+        assert all(torch.equal(a, b) for a, b in zip(plain, want))
+    seen = []
+    handles = [D.gamma.register_hook(lambda g: g * 2), D.slope.register_post_accumulate_grad_hook(lambda p: seen.append(p))]
+    got = back()
+    assert torch.equal(got[0], plain[0] * 2) and torch.equal(got[1], plain[1]) and torch.equal(got[2], plain[2])
+    assert len(seen) == 1 and seen[0] is D.slope
+    for h in handles:
+        h.remove()
+    assert all(torch.equal(a, b) for a, b in zip(back(), plain)) and len(seen) == 1

@@ -1249,3 +1249,28 @@ def test_flat_gradients_across_streams(ops, where):
     got[nb] = want[nb]
     assert torch.equal(got, want)
     assert m.w.grad.data_ptr() == flat.grad.data_ptr()
+
+
+def test_flat_gradients_with_hooks(ops):
+    """Gradient hooks of parameters in the flat buffer run, and what they return is what arrives there."""
+    from gan_amd.optim import FusedAdamW
+    m = _ConvPReLU().to(DEV)
+    flat = FusedAdamW(m).flat
+    geo = ops.conv_geo(4, 6, 16, 16, 8, 3, 1, 1)
+    x = torch.randn(6, 4, 16, 16, generator=torch.Generator().manual_seed(4)).to(DEV)
+    gy = torch.randn(8, 4, 16, 16, generator=torch.Generator().manual_seed(5)).to(DEV)
+    call = lambda: ops.prelu(ops.conv2d(x, m.w, m.b, geo, 1.0), m.a)   # noqa: E731
+    call().backward(gy)
+    want = flat.grad.clone()
+    seen = []
+    handles = [m.w.register_hook(lambda g: g * 2), m.a.register_post_accumulate_grad_hook(lambda p: seen.append(p))]
+    flat.grad.zero_()
+    call().backward(gy)
+    n = m.w.numel()
+    assert torch.equal(flat.grad[:n], want[:n] * 2) and torch.equal(flat.grad[n:], want[n:])
+    assert len(seen) == 1 and seen[0] is m.a
+    for h in handles:
+        h.remove()
+    flat.grad.zero_()
+    call().backward(gy)
+    assert torch.equal(flat.grad, want) and len(seen) == 1
