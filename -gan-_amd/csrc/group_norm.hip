@@ -270,6 +270,8 @@ int ganamd_group_norm_fwd(const ganamd_norm_desc* d, const void* x, const void* 
   if (!make_plan(d, gn::FWD, f) || !x || !y || !stats || (d->act == GANAMD_NORM_PRELU && !slope) ||
       workspace_bytes < f.total || (f.total && !workspace))
     return GANAMD_EINVAL;
+  // in place, no elementwise block may read a pivot that another one has overwritten: a group kernel goes before
+  if (x == y) f.p.fold_apply = false;
   Args a = f.a;
   a.x = x; a.w = w; a.b = b; a.slope = d->act == GANAMD_NORM_PRELU ? slope : nullptr;
   a.o1 = y; a.stats = stats;

@@ -303,6 +303,7 @@ int ganamd_group_norm_workspace(const ganamd_norm_desc* d, int op, size_t* bytes
  * planes per block, positions in flight, channels per tile, tiles, chunks, positions per chunk of the
  * sums, and of the elementwise pass} (introspection for tests). */
 int ganamd_group_norm_plan_info(const ganamd_norm_desc* d, int op, int* info);
+/* y may be x. */
 int ganamd_group_norm_fwd(const ganamd_norm_desc* d, const void* x, const void* w, const void* b, const void* slope,
                           void* y, double* stats, void* workspace, size_t workspace_bytes, hipStream_t stream);
 /* Any output may be NULL (not wanted).  accumulate: gw, gb, gslope are added to (gx is written). */

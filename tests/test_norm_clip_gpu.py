@@ -1164,3 +1164,23 @@ def test_group_norm_flat_gradients_with_hooks(ops, order):
     for h in handles:
         h.remove()
     assert all(torch.equal(a, b) for a, b in zip(back(), plain)) and len(seen) == 1
+
+
+@pytest.mark.parametrize("shape,G,layout", [((3, 5, 5, 12), 3, "nhwc"), ((64, 40, 37, 12), 4, "nhwc"), ((1, 200_000, 8), 2, "nhwc"),
+                                            ((2, 9, 4100), 4, "nhwc"), ((12, 3, 37), 3, "cnhw"), ((4, 1, 40_000), 2, "cnhw")])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_group_norm_forward_in_place_abi(ops, shape, G, layout, dtype):
+    """The C entry point with y = x."""
+    from gan_amd import _lib
+    t = make(shape, layout, "silu", dtype, 39)
+    want = ops.group_norm_act(t["x"], G, t["w"], t["b"], act="silu", layout=layout)
+    B, C = (shape[0], shape[-1]) if layout == "nhwc" else (shape[1], shape[0])
+    d = _lib.NormDesc(math.prod(shape) // (B * C), B, C, G, ("nhwc", "cnhw").index(layout), (F32, BF16).index(dtype), 0, 1, 0.0, 1e-5)
+    n = _lib.c_size_t(0)
+    assert _lib.LIB.ganamd_group_norm_workspace(d, 0, n) == 0
+    ws = torch.empty(n.value // 4 + 1, device=DEV)
+    stats = torch.empty(B, G, 2, dtype=torch.float64, device=DEV)
+    x = t["x"].clone()
+    assert _lib.LIB.ganamd_group_norm_fwd(d, x.data_ptr(), t["w"].data_ptr(), t["b"].data_ptr(), None, x.data_ptr(),
+                                          stats.data_ptr(), ws.data_ptr(), ws.numel() * 4, _lib.stream()) == 0
+    assert torch.equal(x, want)
